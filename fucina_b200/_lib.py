@@ -21,6 +21,13 @@ class QmmTile(C.Structure):
     _fields_ = [("expert", C.c_int32), ("base_row", C.c_int32), ("m", C.c_int32), ("tile_m", C.c_int32)]
 
 
+class KvPagesStruct(C.Structure):
+    """`fq_kv_pages`: where the pages of a key-value cache lie and how they are laid out."""
+
+    _fields_ = [("fmt", C.c_int), ("k", c_void), ("v", c_void), ("k_scale", c_void), ("v_scale", c_void), ("n_pages", c_size),
+                ("page_tokens", c_size), ("kv_heads", c_size), ("d", c_size), ("page_stride", c_size), ("scale_stride", c_size)]
+
+
 # name -> (restype, argtypes); mirrors include/fucina_b200.h one to one
 SIGNATURES = {
     "fq_init": (c_int, [c_int]),
@@ -91,6 +98,8 @@ SIGNATURES = {
     "fq_ep_emulate_for_test": (c_int, [c_int, P(c_void), P(c_void), P(c_void), P(c_void), c_size, c_size, P(c_void), P(c_void), P(c_void),
                                        c_size, c_int]),
     "fq_router_topk_dev": (c_int, [c_void, c_size, c_size, c_size, c_int, c_void, c_void, c_void]),
+    "fq_router_groups_dev": (c_int, [c_void, c_size, c_size, c_int, c_void, c_size, c_size, c_int, c_size, c_int, C.c_float, c_void, c_void,
+                                     c_void]),
     "fq_should_use_gpu_dense_quant": (c_int, [c_int, c_u64]),
     "fq_should_use_gpu_dense_quant_packed": (c_int, [c_int, c_u64]),
     "fq_should_use_gpu_quant_decode": (c_int, [c_int, c_size, c_size, c_size]),
@@ -105,6 +114,11 @@ SIGNATURES = {
                                 C.c_float, c_size, c_int, c_void]),
     "fq_attn_fwd": (c_int, [c_void, c_void, c_void, c_int, c_void, c_void, c_void, c_size, c_size, c_size, c_size, c_size, c_size, C.c_float,
                             c_size, c_int]),
+    "fq_kv_append_dev": (c_int, [P(KvPagesStruct), c_void, c_void, c_size, c_void, c_void, c_size, c_void, c_size, c_size, c_void]),
+    "fq_kv_read_dev": (c_int, [P(KvPagesStruct), c_void, c_void, c_int, c_void, c_void, c_size, c_void, c_size, c_size, c_void]),
+    "fq_attn_paged_workspace_bytes": (c_size, [P(KvPagesStruct), c_size, c_size, c_size]),
+    "fq_attn_paged_dev": (c_int, [P(KvPagesStruct), c_void, c_size, c_void, c_void, c_size, c_size, c_size, c_size, C.c_float, c_size, c_void,
+                                  c_void, c_void, c_size, c_void]),
     "fq_gguf_open": (c_int, [C.c_char_p, P(c_void)]),
     "fq_gguf_close": (None, [c_void]),
     "fq_gguf_tensor_count": (c_size, [c_void]),

@@ -198,6 +198,7 @@ int device_status(Ctx* ctx) {
     if (s == 0) return FQ_OK;
     *(volatile int*)ctx->status_host = 0;
     if (s == FQ_ERR_CAPACITY) return fail(s, "the routing sent a GPU more rows than its exchange arena holds");
+    if (s == FQ_ERR_PAGE) return fail(s, "a page table entry, sequence, position or length named something outside the key-value cache");
     return fail(s, "a device-side wait gave up (status %d)", s);
 }
 

@@ -15,7 +15,7 @@ import os
 import numpy as np
 
 from . import formats
-from ._lib import QmmTile, load
+from ._lib import KvPagesStruct, QmmTile, load
 
 MODE_AUTO, MODE_INT8, MODE_TENSOR = 0, 1, 2
 
@@ -192,6 +192,51 @@ def attn_fwd_dev(q_dev, k_dev, v_dev, kv_is_f16: bool, out_dev, kvmap_dev, q_seq
                  source_offset: int, scale: float, window: int = 0, causal: bool = True, stats_dev=None, stream: int = 0) -> None:
     _check(load().fq_attn_fwd_dev(_vp(q_dev), _vp(k_dev), _vp(v_dev), int(kv_is_f16), _vp(out_dev), _vp(stats_dev), _vp(kvmap_dev), q_seq,
                                   kv_seq, heads, kv_heads, d, source_offset, scale, window, int(causal), C.c_void_p(stream)))
+
+
+# --------------------------------------------------------------------------- paged key-value cache
+KV_F16, KV_Q8_0 = 0, 1
+
+
+class KvPages:
+    """Pages of a key-value cache in the caller's device memory (`fq_kv_pages`): k, v [n_pages][kv_heads][page_tokens][d]
+    f16 or int8, for KV_Q8_0 with k_scale, v_scale [n_pages][kv_heads][page_tokens][d / 32] f16. The object keeps the four
+    buffers alive; strides are elements from page to page (0 = dense)."""
+
+    __slots__ = ("struct", "ref", "_keep")
+
+    def __init__(self, fmt: int, k, v, k_scale, v_scale, n_pages: int, page_tokens: int, kv_heads: int, d: int, page_stride: int = 0,
+                 scale_stride: int = 0):
+        self.struct = KvPagesStruct(fmt, _vp(k), _vp(v), _vp(k_scale), _vp(v_scale), n_pages, page_tokens, kv_heads, d, page_stride, scale_stride)
+        self.ref = C.byref(self.struct)
+        self._keep = (k, v, k_scale, v_scale)
+
+
+def kv_append_dev(pages: KvPages, k_dev, v_dev, token_seq_dev, token_pos_dev, n_tokens: int, page_table_dev, n_seqs: int, max_pages: int,
+                  row_stride: int = 0, stream: int = 0) -> None:
+    """Rows of f32 keys and values into their pages (`fq_kv_append_dev`); rows with token_seq < 0 are skipped."""
+    _check(load().fq_kv_append_dev(pages.ref, _vp(k_dev), _vp(v_dev), row_stride, _vp(token_seq_dev), _vp(token_pos_dev), n_tokens,
+                                   _vp(page_table_dev), n_seqs, max_pages, C.c_void_p(stream)))
+
+
+def kv_read_dev(pages: KvPages, k_out_dev, v_out_dev, out_is_f16: bool, token_seq_dev, token_pos_dev, n_tokens: int, page_table_dev,
+                n_seqs: int, max_pages: int, stream: int = 0) -> None:
+    """Rows of the cache as dense f32 or f16 rows (`fq_kv_read_dev`), the K and V operands of `attn_fwd_dev`."""
+    _check(load().fq_kv_read_dev(pages.ref, _vp(k_out_dev), _vp(v_out_dev), int(out_is_f16), _vp(token_seq_dev), _vp(token_pos_dev), n_tokens,
+                                 _vp(page_table_dev), n_seqs, max_pages, C.c_void_p(stream)))
+
+
+def attn_paged_workspace_bytes(pages: KvPages, n_seqs: int, heads: int, max_len: int) -> int:
+    """Device bytes `attn_paged_dev` works in for these sizes (0: none needed, or sizes it declines)."""
+    return int(load().fq_attn_paged_workspace_bytes(pages.ref, n_seqs, heads, max_len))
+
+
+def attn_paged_dev(pages: KvPages, q_dev, out_dev, page_table_dev, kv_len_dev, n_seqs: int, max_pages: int, heads: int, scale: float,
+                   window: int = 0, max_len: int = 0, q_stride: int = 0, stats_dev=None, workspace=None, workspace_bytes: int = 0,
+                   stream: int = 0) -> None:
+    """Attention of one new token per sequence over its pages (`fq_attn_paged_dev`): q, out [n_seqs][heads][d] f32."""
+    _check(load().fq_attn_paged_dev(pages.ref, _vp(q_dev), q_stride, _vp(page_table_dev), _vp(kv_len_dev), n_seqs, max_pages, max_len, heads,
+                                    scale, window, _vp(out_dev), _vp(stats_dev), _vp(workspace), workspace_bytes, C.c_void_p(stream)))
 
 
 class _GgufTensor(C.Structure):
@@ -584,6 +629,18 @@ def router_topk_dev(logits_dev, seq: int, n_expert: int, top_k: int, normalize: 
     """`routerTopK` (src/exec/topk.zig:21-86) on the device."""
     _check(load().fq_router_topk_dev(_vp(logits_dev), seq, n_expert, top_k, int(normalize), _vp(selected_dev),
                                      _vp(weights_dev), C.c_void_p(stream)))
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
+
+
+def router_groups_dev(logits_dev, seq: int, n_expert: int, top_k: int, selected_dev, weights_dev, score: int = SCORE_SOFTMAX, bias_dev=None,
+                      n_group: int = 1, topk_group: int = 1, group_score: int = GROUP_MAX, normalize: bool = True, scale: float = 1.0,
+                      stream: int = 0) -> None:
+    """Expert choice by softmax or sigmoid scores with a balance bias and expert groups (`fq_router_groups_dev`)."""
+    _check(load().fq_router_groups_dev(_vp(logits_dev), seq, n_expert, score, _vp(bias_dev), n_group, topk_group, group_score, top_k,
+                                       int(normalize), scale, _vp(selected_dev), _vp(weights_dev), C.c_void_p(stream)))
 
 
 # --------------------------------------------------------------------------- gates

@@ -59,7 +59,8 @@ enum {
     FQ_DECLINED_BUSY = 5,    /* all async slots in flight */
     FQ_ERR_CUDA = -1,
     FQ_ERR_TIMEOUT = -2,     /* a bounded device-side wait gave up */
-    FQ_ERR_CAPACITY = -3     /* the routing sent more rows to a GPU than its exchange arena holds */
+    FQ_ERR_CAPACITY = -3,    /* the routing sent more rows to a GPU than its exchange arena holds */
+    FQ_ERR_PAGE = -4         /* a page table entry, sequence, position or length named something outside the cache */
 };
 
 /* backend/ops.zig:89-107 `GatedOp`: g = source(up) * activation(gate) (ops.zig:150-190).
@@ -158,6 +159,63 @@ FQ_API int fq_attn_fwd_dev(const float* q_dev, const void* k_dev, const void* v_
 FQ_API int fq_attn_fwd(const float* q, const void* k, const void* v, int kv_is_f16, float* out, float* stats,
                        const int32_t* kv_head_for_head, size_t q_seq, size_t kv_seq, size_t heads, size_t kv_heads, size_t d,
                        size_t source_offset, float scale, size_t window, int causal);
+
+/* ---- paged key-value cache (new: the reference keeps one contiguous f16 or f32 cache per sequence) ----
+ * Pages of page_tokens tokens (a multiple of 16) in the caller's device memory; a page holds all kv heads, one head's
+ * tokens next to each other:
+ *   k, v              [n_pages][kv_heads][page_tokens][d]       f16 (FQ_KV_F16) or int8 (FQ_KV_Q8_0)
+ *   k_scale, v_scale  [n_pages][kv_heads][page_tokens][d / 32]  f16, FQ_KV_Q8_0 only (NULL otherwise)
+ * FQ_KV_Q8_0 follows the Q8_0 block law of fq_quantize_acts_q8_0_dev (q8k.zig:49-69): 32 values share a scale, a value
+ * is scale * level; blocks are bit-identical to that encoder's. FQ_KV_F16 rounds once to f16 (beyond its range:
+ * infinity). d <= 256, a multiple of 16 (f16) or 32 (Q8_0); kv_heads <= 512; page_tokens <= 4096.
+ * page_stride / scale_stride: elements from one page to the next in k, v / in the scales, 0 for dense pages; larger
+ * strides let the pages of several layers, or K and V, interleave in one allocation. Pointers are 16-byte aligned and
+ * the strides keep every page so.
+ * A page table [n_seqs][max_pages] int32 on the device names the pages of each sequence in order: position p of
+ * sequence s lives in page table[s][p / page_tokens]. Sequences may share pages they only read. Entries behind a
+ * sequence's length are never read. What lies in slots that no call wrote is never used, NaN included.
+ * A page id outside [0, n_pages), a position behind the table's end or a sequence outside [0, n_seqs) touches no
+ * memory: that row is skipped (append, read: left as it was; attention: the keys do not take part) and the next
+ * fq_synchronize or blocking entry returns FQ_ERR_PAGE once. */
+enum { FQ_KV_F16 = 0, FQ_KV_Q8_0 = 1 };
+typedef struct {
+    int fmt; /* FQ_KV_* */
+    void* k;
+    void* v;
+    void* k_scale;
+    void* v_scale;
+    size_t n_pages, page_tokens, kv_heads, d;
+    size_t page_stride, scale_stride;
+} fq_kv_pages;
+/* Write n_tokens rows of keys and values: row r is position token_pos[r] of sequence token_seq[r]; rows with
+ * token_seq < 0 (padding) are skipped. k_dev and v_dev are f32 [n_tokens][kv_heads * d] with row_stride elements
+ * between rows (0 = dense; a multiple of 4), so both may point into the rows of a fused projection. No two rows of a
+ * call may name the same slot. n_tokens 0 does nothing. Neither allocates nor synchronises. */
+FQ_API int fq_kv_append_dev(const fq_kv_pages* pages, const float* k_dev, const float* v_dev, size_t row_stride,
+                            const int32_t* token_seq_dev, const int32_t* token_pos_dev, size_t n_tokens, const int32_t* page_table_dev,
+                            size_t n_seqs, size_t max_pages, void* stream);
+/* Read rows back in any order: k_out_dev and v_out_dev [n_tokens][kv_heads][d] f32, or f16 (out_is_f16 != 0, rounded
+ * once): the K and V operands of fq_attn_fwd_dev when a prompt chunk attends to what its sequence has cached. Either
+ * output may be NULL. Rows with token_seq < 0 are left as they were. Neither allocates nor synchronises. */
+FQ_API int fq_kv_read_dev(const fq_kv_pages* pages, void* k_out_dev, void* v_out_dev, int out_is_f16, const int32_t* token_seq_dev,
+                          const int32_t* token_pos_dev, size_t n_tokens, const int32_t* page_table_dev, size_t n_seqs, size_t max_pages,
+                          void* stream);
+/* Attention of one new token per sequence over its pages (the decode step of fq_attn_fwd_dev for a batch of sequences
+ * with lengths of their own): q_dev [n_seqs][heads][d] f32 with q_stride elements between sequences (0 = dense; a
+ * multiple of 4), out_dev [n_seqs][heads][d] f32. Query head h reads kv head h / (heads / kv_heads). Sequence s sees
+ * the keys [max(0, len - window), len) with len = kv_len_dev[s] (window 0: all; append the new token first, it counts).
+ * out = softmax(scale * q.k) v, f32 accuracy throughout; a sequence of length 0 gets zeros. Optional stats_dev
+ * [n_seqs][heads][2] = {row max, sum exp} (a length of 0: {-3.4e38, 0}).
+ * max_len: the longest length that may occur (0 = max_pages * page_tokens); longer lengths count as max_len and leave
+ * FQ_ERR_PAGE. It sizes the workspace and picks the split, so a replayed graph serves every length up to it.
+ * workspace_dev: fq_attn_paged_workspace_bytes of device memory, 16-byte aligned, contents irrelevant before and after;
+ * one call at a time may use it (two graphs that may run at the same time need one each). NULL: taken from the
+ * library's caching allocator for the call (declined while the stream is being captured). Same inputs give the same
+ * bits whatever else runs. heads <= 4096, n_seqs <= 65535. */
+FQ_API size_t fq_attn_paged_workspace_bytes(const fq_kv_pages* pages, size_t n_seqs, size_t heads, size_t max_len);
+FQ_API int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_stride, const int32_t* page_table_dev,
+                             const int32_t* kv_len_dev, size_t n_seqs, size_t max_pages, size_t max_len, size_t heads, float scale,
+                             size_t window, float* out_dev, float* stats_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /* ---- GGUF file -> device-resident weights (new on the GPU side). The reference parses GGUF in src/gguf.zig
  *      (:214-452: header, metadata, tensor table, data section aligned to general.alignment) and makes quantized
@@ -377,6 +435,25 @@ FQ_API int fq_ep_emulate_for_test(int world, const fq_weights* const* gate, cons
 /* exec/topk.zig:21-86 `routerTopK` on the device: logits [seq, E] -> selected/weights [seq, top_k]. */
 FQ_API int fq_router_topk_dev(const float* logits_dev, size_t seq, size_t n_expert, size_t top_k, int normalize,
                        int32_t* selected_dev, float* weights_dev, void* stream);
+
+/* Router with expert groups (new; the reference's router is the softmax top-k above): logits [seq][n_expert] f32 ->
+ * selected / weights [seq][top_k], ready for fq_moe_layer_dev.
+ *   score   softmax over the row or sigmoid per expert (FQ_SCORE_*)
+ *   key     score + bias_dev[expert] (NULL: the score alone): decides who is chosen, never the weight
+ *   groups  n_group equal runs of experts; the topk_group groups with the best rank stay open, rank = the group's best
+ *           key or the sum of its two best (FQ_GROUP_*; a group of one expert: its key)
+ *   chosen  the top_k best keys among the open groups, best first; equal keys and ranks go to the lowest index
+ *   weight  the chosen score, divided by the chosen scores' sum when normalize != 0 and that sum is positive, times
+ *           scale
+ * Keys and ranks are compared as 64-bit numbers, so experts closer than f32 resolves are still told apart. A logit of
+ * -infinity or NaN closes its expert (key -infinity, weight 0); when fewer than top_k open experts remain, closed ones
+ * follow by index. n_expert <= 4096, top_k <= 32, top_k <= topk_group * (n_expert / n_group), n_group <= 64.
+ * Neither allocates nor synchronises. */
+enum { FQ_SCORE_SOFTMAX = 0, FQ_SCORE_SIGMOID = 1 };
+enum { FQ_GROUP_MAX = 0, FQ_GROUP_TOP2 = 1 };
+FQ_API int fq_router_groups_dev(const float* logits_dev, size_t seq, size_t n_expert, int score, const float* bias_dev, size_t n_group,
+                                size_t topk_group, int group_score, size_t top_k, int normalize, float scale, int32_t* selected_dev,
+                                float* weights_dev, void* stream);
 
 /* ---- gates (backend/cuda.zig:2494-2554) and test seams (:2537-2571) ---- */
 FQ_API int fq_should_use_gpu_dense_quant(int fmt, uint64_t total_work);
