@@ -211,7 +211,7 @@ FQ_API int fq_kv_read_dev(const fq_kv_pages* pages, void* k_out_dev, void* v_out
  * workspace_dev: fq_attn_paged_workspace_bytes of device memory, 16-byte aligned, contents irrelevant before and after;
  * one call at a time may use it (two graphs that may run at the same time need one each). NULL: taken from the
  * library's caching allocator for the call (declined while the stream is being captured). Same inputs give the same
- * bits whatever else runs. heads <= 4096, n_seqs <= 65535. */
+ * bits whatever else runs. heads <= 4096, n_seqs <= 65535, max_len <= 2^28. */
 FQ_API size_t fq_attn_paged_workspace_bytes(const fq_kv_pages* pages, size_t n_seqs, size_t heads, size_t max_len);
 FQ_API int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_stride, const int32_t* page_table_dev,
                              const int32_t* kv_len_dev, size_t n_seqs, size_t max_pages, size_t max_len, size_t heads, float scale,
