@@ -8,19 +8,23 @@
 //
 // Bound: HBM, the cache bytes of the keys in range; everything below serves to keep those copies in flight.
 //
-// Split. Work is counted in units of 16 keys of one kv head (a unit never straddles pages); a row is one (sequence, kv
-// head). All units of all rows, in order, are cut into equal shares, one per ring: uneven lengths load the GPU evenly and
-// one long sequence uses all of it. A ring is a few shared-memory stages of one unit each, filled by cp.async and walked by
-// 1 to 4 warps, each with up to eight of the query heads that share the kv head. A row that lies inside one ring's share
-// is finished there; pieces of rows that cross shares are joined inside the CTA in shared memory, and pieces that cross
-// CTAs go to the workspace and are joined, in order, by a second kernel. When every row is short, one CTA takes one row
-// and no second kernel runs. The lengths are read on the device: nothing on the host depends on them.
+// Split. Work is counted in units of 32 keys (16 where a row of K is longer than 128 values) of one kv head; a row is one
+// (sequence, kv head). All units of all rows, in order, are cut into equal shares, one per ring: uneven lengths load the
+// GPU evenly and one long sequence uses all of it. A ring is two or three shared-memory stages of one unit each, filled by
+// cp.async and walked by 1 to 4 warps, each with up to eight of the query heads that share the kv head. A row that lies
+// inside one ring's share is finished there; pieces of rows that cross shares are joined inside the CTA, and pieces that
+// cross CTAs go to the workspace and are joined, in order, by a second kernel. When every row is short, one CTA takes one
+// row and no second kernel runs. The lengths are read on the device: nothing on the host depends on them.
+//
+// Copies. The keys of a stage are refilled as soon as the scores are taken, the values after the second product: nearly
+// two units per ring are in flight at any time from two stages' room.
 //
 // Arithmetic. mma.sync m16n8k16 on f16 operands with f32 sums, at f32 accuracy: the operand with 16 rows holds eight heads
 // twice, rows 0-7 the leading f16 part of each f32 value and rows 8-15 the remainder (22 bits together), so query and
-// weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16. Query rows are
-// scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's smallest steps.
-// Q8_0 scales multiply the f32 sums of a 32-value block of a score, and the f32 weights before they are split.
+// weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16. Query
+// rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's
+// smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a value's scale s turns the two parts
+// (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'), whose bracket is exact in f16.
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -33,12 +37,16 @@ namespace {
 
 constexpr float kNegBig = -3.4e38f;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kUnit = 16;      // keys per unit
+constexpr int kSub = 16;       // keys that surely lie in one page
 constexpr int kRowsPerWarp = 8;
-constexpr int kMaxWarps = 8;   // per CTA: up to 255 registers a thread
-constexpr int kMaxStages = 8;
+constexpr int kMaxRings = 16;  // 2 x kMaxRings pieces are joined by one lane each
 constexpr int kSmemMost = 226 * 1024;
 constexpr size_t kMaxLen = (size_t)1 << 28;
+
+// Keys per unit and warps per CTA for rows of up to `dm` values: what the registers (o is dm / 2 of them, the query as
+// many as a quarter of that again) and the stages' room allow.
+__host__ __device__ constexpr int unit_keys(int dm) { return dm <= 128 ? 32 : 16; }
+__host__ __device__ constexpr int max_warps(int dm) { return dm <= 64 ? 12 : 8; }
 
 struct PagedArgs {
     KvView c;
@@ -58,26 +66,19 @@ struct PagedArgs {
     int stage_bytes;
     int row_mode;      // one CTA per row; else shares of at least min_units
     int min_units;
-    unsigned long long page_magic;  // unit / units per page = unit * page_magic >> 32
-    int* meta;         // [grid][2]: the row whose first piece CTA c holds in part 1 (-1: none), the last CTA with a piece of it (in part 0)
-    float* parts;      // [grid][2][warps_per_ring * 8][d + 2]: o, then max and sum
+    unsigned long long page_magic;  // (16 keys) / (16 keys of a page) = x * page_magic >> 32
+    int* meta;         // [grid][2]: the row whose beginning CTA c holds in part 1 (-1: none), the last CTA with a piece of it (in part 0)
+    float* parts;      // [grid][2 + rings][warps_per_ring * 8][d + 2]: o, then max and sum; part 2 + r: the first piece of ring r
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// all but the newest `newer` groups have landed
-__device__ __forceinline__ void cp_async_wait(int newer) {
-    switch (newer) {
-        case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-        case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-        case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-        case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-        case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-        case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-        default: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    }
+// the oldest of the 2 * stages groups under way has landed
+__device__ __forceinline__ void cp_async_wait_oldest(int stages) {
+    if (stages == 2) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else asm volatile("cp.async.wait_group 5;" ::: "memory");
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -90,25 +91,36 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// the same into fresh sums
+__device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 // x, y as f16 leading parts and remainders
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&r);
+    hi = bits_of(h), lo = bits_of(__floats2half2_rn(x - f.x, y - f.y));
+}
+// A sum over both halves of the 16-row operand. Where the leading part met an infinity the remainder's product is
+// meaningless (0 or a negative number times infinity).
+__device__ __forceinline__ float whole(float lead, float rest) {
+    const float x = lead + rest;
+    return x != x ? lead : x;
 }
 // Two of a word's four int8 values as f16: byte b + 128 becomes the low mantissa bits of 1024 + (b + 128); subtracting 1152
 // is exact. sel 0x4140 takes bytes 0 and 1, 0x4342 bytes 2 and 3, 0x4240 the even and 0x4341 the odd ones.
 template <int SEL>
 __device__ __forceinline__ uint32_t widen(uint32_t biased) {
-    const uint32_t u = __byte_perm(biased, 0x64646464u, SEL);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    return bits_of(__hsub2(half2_of(__byte_perm(biased, 0x64646464u, SEL)), half2_of(0x64806480u)));
 }
 
 // The keys sequence s sees; a length the call does not allow is cut and reported.
@@ -120,15 +132,19 @@ __device__ __forceinline__ void key_range(const PagedArgs& A, int s, int& first,
     }
     first = (A.window > 0 && end > A.window) ? end - A.window : 0;
 }
-// Units of a row of sequence s: at least one, so that an empty sequence has somebody to write its zeros.
-__device__ __forceinline__ int units_of(int first, int end) { return max(1, (end + kUnit - 1) / kUnit - first / kUnit); }
+// Units of a row: at least one, so that an empty sequence has somebody to write its zeros.
+template <int UK>
+__device__ __forceinline__ int units_of(int first, int end) {
+    return max(1, (end + UK - 1) / UK - first / UK);
+}
 
 // Where a ring stands: unit `u` of row `r` of sequence `s`.
+template <int UK>
 struct Cursor {
     int s, r, u, units, first, end;
     __device__ __forceinline__ void load(const PagedArgs& A) {
         key_range(A, s, first, end);
-        units = units_of(first, end);
+        units = units_of<UK>(first, end);
     }
     __device__ __forceinline__ void next(const PagedArgs& A, int rows_per_seq) {
         if (++u < units) return;
@@ -139,42 +155,59 @@ struct Cursor {
     }
 };
 
-// Partial results of a row inside the CTA: two per ring, one of a row that began in an earlier share and one of a row
-// that began here and ends in a later one.
+// Partial results of a row inside the CTA: two per ring, one of a row that began in an earlier share (kept in the
+// workspace; with a CTA per row, on the ring's stages, like the other) and one of a row that began here and ends later.
 struct Piece {
     int row;   // -1: none
     int last;  // the CTA that holds the row's last unit; -1: the unit is in this piece
 };
 
-// A sum over both halves of the 16-row operand. Where the leading part met an infinity the remainder's product is
-// meaningless (0 or a negative number times infinity).
-__device__ __forceinline__ float whole(float lead, float rest) { return fabsf(lead) == INFINITY ? lead : lead + rest; }
+// The scales of one key (or value) row: nb = d / 32 halves, in registers as pairs.
+template <int NB, bool EXACT>
+__device__ __forceinline__ void load_scales(const __half* row, int nb, uint32_t (&w)[(NB + 1) / 2]) {
+    if (EXACT && NB == 2) {
+        w[0] = *reinterpret_cast<const uint32_t*>(row);
+    } else if (EXACT && NB == 4) {
+        const uint2 x = *reinterpret_cast<const uint2*>(row);
+        w[0] = x.x, w[1] = x.y;
+    } else if (EXACT && NB == 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row);
+        w[0] = x.x, w[1] = x.y, w[2 % ((NB + 1) / 2)] = x.z, w[3 % ((NB + 1) / 2)] = x.w;
+    } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+        for (int i = 0; i < (NB + 1) / 2; ++i) w[i] = (2 * i < nb ? h[2 * i] : 0u) | (2 * i + 1 < nb ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+    }
+}
 
-template <bool Q8, int DM>
-__global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const PagedArgs A) {
+// EXACT: rows have DM values; else up to DM
+template <bool Q8, int DM, bool EXACT>
+__global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const __grid_constant__ PagedArgs A) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Piece sh_piece[kMaxWarps][2];
+    __shared__ Piece sh_piece[kMaxRings][2];
     pdl_wait_then_release();
-    constexpr int KS = DM / 16;  // 16-value steps of a row
+    constexpr int UK = unit_keys(DM), NT = UK / 8;  // keys of a unit, and groups of eight of them
+    constexpr int KS = DM / 16, NB = DM / 32;       // 16-value steps and 32-value blocks of a row
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int ring = warp / A.warps_per_ring, part = warp - ring * A.warps_per_ring;
-    const int d = A.c.d, steps = d >> 4;
-    const int nc = Q8 ? d >> 4 : d >> 3;   // 16-byte chunks of a key's row
-    const int pitch = (nc + 1) * 16;       // an odd number of chunks: the rows of an ldmatrix fall on distinct banks
+    const int d = EXACT ? DM : A.c.d, steps = d >> 4, nb = d >> 5;
+    const int nc = Q8 ? d >> 4 : d >> 3;  // 16-byte chunks of a key's row
+    const int pitch = (nc + 1) * 16;      // an odd number of chunks: the rows of an ldmatrix fall on distinct banks
     const int rows_per_seq = A.c.kv_heads * A.passes;
     const int prow = A.warps_per_ring * kRowsPerWarp;  // head rows of a piece
     const int piece_floats = prow * (d + 2);
-    // shared memory: the rings' stages, then one piece per ring; a ring's other piece goes where its stages were
+    // a stage: K rows, V rows, and for Q8_0 their scales [UK][d / 32]
+    const int k_scale_at = 2 * UK * pitch, v_scale_at = k_scale_at + UK * 2 * nb;
     uint8_t* ring_base = smem + (size_t)ring * A.stages * A.stage_bytes;
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring_base);
-    float* pieces_a = reinterpret_cast<float*>(smem + (size_t)A.rings * A.stages * A.stage_bytes);
     auto piece_ptr = [&](int rg, int which) {
-        return which == 0 ? pieces_a + (size_t)rg * piece_floats : reinterpret_cast<float*>(smem + (size_t)rg * A.stages * A.stage_bytes);
+        return which == 0 && !A.row_mode ? A.parts + ((size_t)blockIdx.x * (2 + A.rings) + 2 + rg) * piece_floats
+                                         : reinterpret_cast<float*>(smem + (size_t)rg * A.stages * A.stage_bytes);
     };
 
     // ---- this ring's share
-    Cursor cur;
+    Cursor<UK> cur;
     int count, share = 1;
     long long from = 0;
     if (A.row_mode) {
@@ -187,7 +220,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
         for (int s = lane; s < A.n_seqs; s += 32) {
             int first, end;
             key_range(A, s, first, end);
-            mine += units_of(first, end);
+            mine += units_of<UK>(first, end);
         }
         const int total = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine) * rows_per_seq;
         const int workers = gridDim.x * A.rings;
@@ -200,7 +233,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
             int before = 0;
             for (int s0 = 0; s0 < A.n_seqs; s0 += 32) {
                 int first = 0, end = 0, n = 0;
-                if (s0 + lane < A.n_seqs) key_range(A, s0 + lane, first, end), n = units_of(first, end) * rows_per_seq;
+                if (s0 + lane < A.n_seqs) key_range(A, s0 + lane, first, end), n = units_of<UK>(first, end) * rows_per_seq;
                 int sum = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -213,7 +246,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
                     const int local = (int)(from - before) - __shfl_sync(0xffffffffu, sum - n, l);
                     cur.s = s0 + l;
                     cur.first = __shfl_sync(0xffffffffu, first, l), cur.end = __shfl_sync(0xffffffffu, end, l);
-                    cur.units = units_of(cur.first, cur.end);
+                    cur.units = units_of<UK>(cur.first, cur.end);
                     cur.r = local / cur.units, cur.u = local - cur.r * cur.units;
                     break;
                 }
@@ -223,56 +256,94 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
     }
     if (part == 0 && lane < 2) sh_piece[ring][lane] = {-1, -1};
 
-    // ---- copies: the ring's warps share the chunks of a unit
-    Cursor ahead = cur;
-    int to_issue = count;
-    int page = -1, page_unit = 0;
-    unsigned bad = 0;  // stages whose unit names no page
+    // ---- copies. `ahead` is the unit copied next, `tok[x]` the place of its x-th 16 keys (tokens of all pages and heads in
+    // storage order; -1: nothing to copy), looked up one step before it is needed. `gone`: per stage and 16 keys, a bit for
+    // keys whose page is no page.
+    Cursor<UK> ahead = cur;
+    int left = count;
+    unsigned gone = 0, gone_next = 0;
+    int pg[UK / kSub], pu[UK / kSub];
+    const int subs_per_page = A.c.page_tokens / kSub;
     auto look_up = [&]() {
-        const int ua = ahead.first / kUnit + ahead.u;
-        const int slot = (int)(((unsigned long long)(unsigned)ua * A.page_magic) >> 32);
-        page_unit = ua - slot * (A.c.page_tokens / kUnit);
-        page = ahead.end > 0 ? A.table[(size_t)ahead.s * A.max_pages + slot] : 0;
+        gone_next = 0;
+#pragma unroll
+        for (int x = 0; x < UK / kSub; ++x) {
+            const int sub = (ahead.first / UK + ahead.u) * (UK / kSub) + x;
+            pg[x] = -1;
+            if (sub * kSub < ahead.end && (sub + 1) * kSub > ahead.first) {
+                const int slot = (int)(((unsigned long long)(unsigned)sub * A.page_magic) >> 32);
+                pu[x] = sub - slot * subs_per_page;
+                pg[x] = A.table[(size_t)ahead.s * A.max_pages + slot];
+            }
+        }
+    };
+    // (after the loads have arrived) which of them name no page
+    auto judge = [&]() {
+#pragma unroll
+        for (int x = 0; x < UK / kSub; ++x) {
+            const int sub = (ahead.first / UK + ahead.u) * (UK / kSub) + x;
+            if (sub * kSub < ahead.end && (sub + 1) * kSub > ahead.first && (pg[x] < 0 || pg[x] >= A.c.n_pages)) {
+                *(volatile int*)A.status = FQ_ERR_PAGE;
+                gone_next |= 1u << x;
+                pg[x] = -1;
+            }
+        }
     };
     const unsigned row_magic = (65536u + nc - 1) / nc;  // chunk / nc = chunk * row_magic >> 16 for chunks < 512
-    auto issue = [&](int stage) {
-        if (to_issue > 0) {
-            const bool ok = page >= 0 && page < A.c.n_pages;
-            bad = ok ? bad & ~(1u << stage) : bad | (1u << stage);
-            if (!ok) {
-                *(volatile int*)A.status = FQ_ERR_PAGE;
-            } else if (ahead.end > 0) {
-                const size_t tok = (size_t)(ahead.r / A.passes) * A.c.page_tokens + (size_t)page_unit * kUnit;
-                const size_t off = ((size_t)page * A.c.page_stride + tok * d) * (Q8 ? 1 : 2);
-                const uint32_t dst = ring_addr + stage * A.stage_bytes;
-                for (int i = part; i < nc; i += A.warps_per_ring) {  // nc / 2 instructions for the keys, as many for the values
-                    const bool side = i >= nc / 2;
-                    const int c = lane + 32 * (side ? i - nc / 2 : i), row = (int)((c * row_magic) >> 16);
-                    cp_async16(dst + (side ? kUnit * pitch : 0) + (c + row) * 16, (side ? A.c.v : A.c.k) + off + (size_t)c * 16);
-                }
-                if (Q8 && part == 0 && lane < 2 * (d >> 4)) {  // 16 keys x d / 32 scales = d bytes a side
-                    const bool side = lane >= d >> 4;
-                    const int c = side ? lane - (d >> 4) : lane;
-                    const size_t so = (size_t)page * A.c.scale_stride + tok * (d >> 5);
-                    cp_async16(dst + 2 * kUnit * pitch + lane * 16, reinterpret_cast<const uint8_t*>((side ? A.c.v_scale : A.c.k_scale) + so) + c * 16);
+    // the keys (side 0) or values of the unit at `ahead` into `stage`
+    auto copy_side = [&](int stage, int side) {
+        if (left > 0) {
+#pragma unroll
+            for (int x = 0; x < UK / kSub; ++x) {
+                if (pg[x] >= 0) {
+                    const size_t tok = (size_t)(ahead.r / A.passes) * A.c.page_tokens + (size_t)pu[x] * kSub;
+                    const size_t off = ((size_t)pg[x] * A.c.page_stride + tok * d) * (Q8 ? 1 : 2);
+                    const uint8_t* src = (side ? A.c.v : A.c.k) + off + lane * 16;
+                    const uint32_t base = ring_addr + stage * A.stage_bytes + (side * UK + x * kSub) * pitch;
+                    if (EXACT) {
+                        // 32 / nc or nc / 32 rows at a time
+                        const uint32_t dst = base + (lane + lane / nc) * 16;
+                        for (int i = part; i < nc / 2; i += A.warps_per_ring) cp_async16(dst + i * (512 + 512 / nc), src + i * 512);
+                    } else {
+                        for (int i = part; i < nc / 2; i += A.warps_per_ring) {
+                            const int c = lane + 32 * i, row = (int)((c * row_magic) >> 16);
+                            cp_async16(base + (c + row) * 16, src + i * 512);
+                        }
+                    }
+                    if (Q8 && part == 0 && lane < nc) {  // 16 keys x d / 32 scales = d bytes
+                        const size_t so = (size_t)pg[x] * A.c.scale_stride + tok * nb;
+                        cp_async16(ring_addr + stage * A.stage_bytes + (side ? v_scale_at : k_scale_at) + x * d + lane * 16,
+                                   reinterpret_cast<const uint8_t*>((side ? A.c.v_scale : A.c.k_scale) + so) + lane * 16);
+                    }
                 }
             }
-            ahead.next(A, rows_per_seq);
-            if (--to_issue > 0) look_up();
         }
         cp_async_commit();
+    };
+    auto step_ahead = [&](int stage) {
+        gone = (gone & ~(3u << (2 * stage))) | gone_next << (2 * stage);
+        if (left > 0) {
+            ahead.next(A, rows_per_seq);
+            if (--left > 0) look_up();
+        }
     };
     auto ring_sync = [&]() {
         if (A.warps_per_ring == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(ring + 1), "r"(A.warps_per_ring * 32) : "memory");
     };
     if (count > 0) look_up();
-    for (int s = 0; s < A.stages - 1; ++s) issue(s);
+    for (int s = 0; s < A.stages; ++s) {
+        if (left > 0) judge();
+        copy_side(s, 0);
+        copy_side(s, 1);
+        step_ahead(s);
+    }
 
     // ---- the share, piece by piece
     uint32_t qa[KS][4];
-    float o[DM / 8][4], l_run = 0.0f, m_run = -INFINITY, row_scale = 1.0f;
-    float v_bound = 0.0f, v_factor = 1.0f;  // Q8_0: values are summed in multiples of the power of two v_bound = 1 / v_factor
+    float o[DM / 8][4], l_run = 0.0f, m_run = -INFINITY, m_use = 0.0f, row_scale = 1.0f;
+    float v_cap = 0.0f, v_unit = 1.0f;  // Q8_0: value scales up to v_cap so far; sums count in multiples of v_unit (a power of two)
+    __half2 v_norm = half2_of(0x3c003c00u);  // 1 / v_unit
     bool started = false;
     int begin_u = 0, stage = 0;
     const int mi = lane >> 3, mr = lane & 7;
@@ -294,7 +365,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
             for (int kk = 0; kk < KS; ++kk) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[kk][i] = 0.0f;
-                if (live && kk < steps) {
+                if (live && (EXACT || kk < steps)) {
                     // f16: columns 2t, 2t + 1, 2t + 8, 2t + 9 of the step; Q8_0: 4t .. 4t + 3, the bytes a lane gets from ldmatrix
                     if (Q8) {
                         const float4 a = *reinterpret_cast<const float4*>(qrow + 16 * kk + 4 * t);
@@ -304,217 +375,252 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
                         x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = b.x, x[kk][3] = b.y;
                     }
                 }
+            }
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[kk][i]));
-            }
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // exponent e of big: rows are multiplied by 2^(14 - e), scores by scale * 2^(e - 14); both factors in two steps so
-            // that neither overflows
+            // exponent e of big: rows are multiplied by 2^(14 - e), scores by scale * 2^(e - 14), each in two steps so that no
+            // factor overflows
             const int e = big > 0.0f && big < INFINITY ? (int)((__float_as_uint(big) >> 23) & 255) - 126 : 0;
-            const float up = __int_as_float((127 + max(-120, min(120, 14 - e))) << 23);
-            const float rest = __int_as_float((127 + (14 - e) - max(-120, min(120, 14 - e))) << 23);
+            const int e1 = max(-120, min(120, 14 - e));
+            const float up = __int_as_float((127 + e1) << 23), rest = __int_as_float((127 + (14 - e) - e1) << 23);
             row_scale = A.scale / up / rest;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
                 split2(x[kk][0] * up * rest, x[kk][1] * up * rest, qa[kk][0], qa[kk][1]);
                 split2(x[kk][2] * up * rest, x[kk][3] * up * rest, qa[kk][2], qa[kk][3]);
             }
-            m_run = -INFINITY, l_run = 0.0f, v_bound = 0.0f, v_factor = 1.0f;
+            m_run = -INFINITY, m_use = 0.0f, l_run = 0.0f, v_cap = 0.0f, v_unit = 1.0f;
 #pragma unroll
             for (int n = 0; n < DM / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         }
-        cp_async_wait(A.stages - 2);
-        ring_sync();  // every warp's copies of this unit have landed, and every warp is done with the stage filled next
-        const bool usable = !((bad >> stage) & 1);
-        issue(stage == 0 ? A.stages - 1 : stage - 1);
+        const int j0 = (cur.first / UK + cur.u) * UK;
+        const int lo = max(cur.first - j0, 0), hi = min(cur.end - j0, UK);
+        const unsigned lost = (gone >> (2 * stage)) & 3;
+        const bool partial = hi - lo < UK || lost;  // some keys do not take part
+        const uint32_t ks = ring_addr + stage * A.stage_bytes, vs = ks + UK * pitch;
+        auto takes_part = [&](int key) { return key >= lo && key < hi && !((lost >> (key / kSub)) & 1); };
 
-        const int j0 = (cur.first / kUnit + cur.u) * kUnit;
-        const int lo = max(cur.first - j0, 0), hi = min(cur.end - j0, kUnit);
-        if (usable && hi > lo) {
-            const uint32_t ks = ring_addr + stage * A.stage_bytes, vs = ks + kUnit * pitch;
-            if (hi - lo < kUnit) {
-                // values outside the range may be anything: their rows (Q8_0: their scales) become zeros. The ring's warps write
-                // the same zeros.
-                uint8_t* rows = ring_base + stage * A.stage_bytes + (Q8 ? 2 * kUnit * pitch + d : kUnit * pitch);
-                const int bytes = Q8 ? (d >> 5) * 2 : d * 2, step = Q8 ? (d >> 5) * 2 : pitch;
-                for (int r = 0; r < kUnit; ++r)
-                    if (r < lo || r >= hi)
-                        for (int i = lane * 2; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(rows + r * step + i) = 0;
-                __syncwarp();
-            }
-            // scores of keys 2t, 2t + 1, 2t + 8, 2t + 9 for head g
-            float sc[4];
-            if (Q8) {
-                sc[0] = sc[1] = sc[2] = sc[3] = 0.0f;
-                const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + 2 * kUnit * pitch);
-                const int nb = d >> 5;
+        // ---- scores: keys 8 n + 2t, + 1 for head g
+        cp_async_wait_oldest(A.stages);
+        ring_sync();  // the keys' copies of all the ring's warps have landed
+        float sc[NT][2];
+        if (Q8) {
+            const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + k_scale_at);
 #pragma unroll
-                for (int b = 0; b < KS / 2; ++b) {
-                    if (b < nb) {
+            for (int n2 = 0; n2 < NT / 2; ++n2) {  // sixteen keys at a time
+                uint32_t w[4][(NB + 1) / 2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) load_scales<NB, EXACT>(ksc + (n2 * 16 + 2 * t + (i & 1) + (i >> 1) * 8) * nb, nb, w[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[2 * n2 + (i >> 1)][i & 1] = 0.0f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    if (EXACT || b < nb) {
                         uint32_t r[4];
-                        ldsm_x4(ks + k_lane + b * 32, r);  // keys 0-7: values 0-15, 16-31 of the block; keys 8-15: the same
-                        float c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0};
+                        ldsm_x4(ks + n2 * 16 * pitch + k_lane + b * 32, r);  // keys 0-7: values 0-15, 16-31 of the block; keys 8-15: the same
+                        float c0[4], c1[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
-                        mma16816(c0, qa[2 * b], widen<0x4140>(r[0]), widen<0x4342>(r[0]));
-                        mma16816(c1, qa[2 * b], widen<0x4140>(r[2]), widen<0x4342>(r[2]));
+                        mma16816_new(c0, qa[2 * b], widen<0x4140>(r[0]), widen<0x4342>(r[0]));
+                        mma16816_new(c1, qa[2 * b], widen<0x4140>(r[2]), widen<0x4342>(r[2]));
                         mma16816(c0, qa[2 * b + 1], widen<0x4140>(r[1]), widen<0x4342>(r[1]));
                         mma16816(c1, qa[2 * b + 1], widen<0x4140>(r[3]), widen<0x4342>(r[3]));
-                        sc[0] = fmaf(__half2float(ksc[(2 * t) * nb + b]), c0[0] + c0[2], sc[0]);
-                        sc[1] = fmaf(__half2float(ksc[(2 * t + 1) * nb + b]), c0[1] + c0[3], sc[1]);
-                        sc[2] = fmaf(__half2float(ksc[(2 * t + 8) * nb + b]), c1[0] + c1[2], sc[2]);
-                        sc[3] = fmaf(__half2float(ksc[(2 * t + 9) * nb + b]), c1[1] + c1[3], sc[3]);
+                        float f[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f[i] = (b & 1) ? __high2float(half2_of(w[i][b / 2])) : __low2float(half2_of(w[i][b / 2]));
+                        sc[2 * n2][0] = fmaf(f[0], c0[0] + c0[2], sc[2 * n2][0]);
+                        sc[2 * n2][1] = fmaf(f[1], c0[1] + c0[3], sc[2 * n2][1]);
+                        sc[2 * n2 + 1][0] = fmaf(f[2], c1[0] + c1[2], sc[2 * n2 + 1][0]);
+                        sc[2 * n2 + 1][1] = fmaf(f[3], c1[1] + c1[3], sc[2 * n2 + 1][1]);
                     }
                 }
-            } else {
-                float c[2][2][4];
+            }
+        } else {
+            float c[NT][4];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) (&c[0][0][0])[i] = 0.0f;
+            for (int kk = 0; kk < KS; ++kk) {
+                if (EXACT || kk < steps) {
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) {
-                    if (kk < steps) {
+                    for (int n2 = 0; n2 < NT / 2; ++n2) {
                         uint32_t r[4];
-                        ldsm_x4(ks + k_lane + kk * 32, r);  // keys 0-7: values 0-7, 8-15 of the step; keys 8-15: the same
-                        mma16816(c[kk & 1][0], qa[kk], r[0], r[1]);
-                        mma16816(c[kk & 1][1], qa[kk], r[2], r[3]);
+                        ldsm_x4(ks + n2 * 16 * pitch + k_lane + kk * 32, r);  // keys 0-7: values 0-7, 8-15 of the step; keys 8-15: the same
+                        if (kk == 0) {
+                            mma16816_new(c[2 * n2], qa[kk], r[0], r[1]);
+                            mma16816_new(c[2 * n2 + 1], qa[kk], r[2], r[3]);
+                        } else {
+                            mma16816(c[2 * n2], qa[kk], r[0], r[1]);
+                            mma16816(c[2 * n2 + 1], qa[kk], r[2], r[3]);
+                        }
                     }
                 }
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int n = i >> 1, x = i & 1;
-                    sc[i] = whole(c[0][n][x] + c[1][n][x], c[0][n][x + 2] + c[1][n][x + 2]);
+            for (int n = 0; n < NT; ++n) sc[n][0] = whole(c[n][0], c[n][2]), sc[n][1] = whole(c[n][1], c[n][3]);
+        }
+        ring_sync();  // all the ring's warps are done with the keys
+        if (left > 0) judge();
+        copy_side(stage, 0);
+
+        // ---- weights
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            sc[n][0] *= row_scale, sc[n][1] *= row_scale;
+            if (partial) {
+                if (!takes_part(8 * n + 2 * t)) sc[n][0] = -INFINITY;
+                if (!takes_part(8 * n + 2 * t + 1)) sc[n][1] = -INFINITY;
+            }
+            top = fmaxf(top, fmaxf(sc[n][0], sc[n][1]));
+        }
+        // the maximum moves rarely after the first units: the sums are touched only then
+        if (__any_sync(0xffffffffu, top > m_run)) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m_run, top);
+            const float r = m_run == -INFINITY ? 0.0f : ex2((m_run - m_new) * kLog2e);
+            m_run = m_new;
+            m_use = m_new == -INFINITY ? 0.0f : m_new;
+            l_run *= r;
+#pragma unroll
+            for (int n = 0; n < DM / 8; ++n) o[n][0] *= r, o[n][1] *= r, o[n][2] *= r, o[n][3] *= r;
+        }
+        uint32_t ph[NT], pl[NT];  // weights times 2^15 of two neighbouring keys, leading parts and remainders
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float p0 = ex2(fmaf(sc[n][0] - m_use, kLog2e, 15.0f)), p1 = ex2(fmaf(sc[n][1] - m_use, kLog2e, 15.0f));
+            l_run += p0 + p1;
+            split2(p0, p1, ph[n], pl[n]);
+        }
+
+        // ---- values
+        cp_async_wait_oldest(A.stages);
+        ring_sync();  // the values' copies have landed
+        if (partial) {
+            // values that do not take part may be anything: their rows (Q8_0: their scales) become zeros. The ring's warps write
+            // the same zeros.
+            uint8_t* rows = ring_base + stage * A.stage_bytes + (Q8 ? v_scale_at : UK * pitch);
+            const int bytes = Q8 ? nb * 2 : d * 2, step = Q8 ? nb * 2 : pitch;
+            for (int r = 0; r < UK; ++r)
+                if (!takes_part(r))
+                    for (int i = lane * 2; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(rows + r * step + i) = 0;
+            __syncwarp();
+        }
+        if (Q8) {
+            const __half* vsc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + v_scale_at);
+            uint32_t w[2 * NT][(NB + 1) / 2];
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) load_scales<NB, EXACT>(vsc + (8 * (i >> 1) + 2 * t + (i & 1)) * nb, nb, w[i]);
+            // 2^15 times a scale above 1 may pass f16's range, and products with scales below 2^-9 lose their remainders to f16's
+            // smallest steps: then the scales are taken relative to a power of two at or above the largest so far
+            __half2 most2 = half2_of(w[0][0]);
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i)
+#pragma unroll
+                for (int b = 0; b < (NB + 1) / 2; ++b) most2 = __hmax2(most2, half2_of(w[i][b]));
+            float most = fmaxf(__low2float(most2), __high2float(most2));
+            if (__any_sync(0xffffffffu, most > v_cap)) {
+#pragma unroll
+                for (int x = 1; x <= 2; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                float unit = 1.0f;
+                v_cap = 1.0f;
+                if (most > 1.0f || most <= 1.0f / 512) {
+                    const unsigned bits = (__float_as_uint(fmaxf(fminf(most, 65536.0f), 1.0f / 32768)) + 0x7fffffu) & 0xff800000u;
+                    unit = v_cap = __uint_as_float(bits);
                 }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = 2 * t + (i & 1) + (i >> 1) * 8;
-                sc[i] = key >= lo && key < hi ? sc[i] * row_scale : -INFINITY;
-                top = fmaxf(top, sc[i]);
-            }
-            // the maximum moves rarely after the first units: the sums are touched only then
-            if (__any_sync(0xffffffffu, top > m_run)) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m_run, top);
-                const float r = m_run == -INFINITY ? 0.0f : ex2((m_run - m_new) * kLog2e);
-                m_run = m_new;
-                l_run *= r;
+                const float r = v_unit / unit;
+                v_unit = unit;
+                v_norm = __float2half2_rn(1.0f / unit);
+                // an earlier unit's sums count in the old unit; the cap never falls
 #pragma unroll
                 for (int n = 0; n < DM / 8; ++n) o[n][0] *= r, o[n][1] *= r, o[n][2] *= r, o[n][3] *= r;
             }
-            float p[4];  // weights times 2^15
+            const bool plain = v_unit == 1.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                p[i] = sc[i] == -INFINITY ? 0.0f : ex2(fmaf(sc[i] - m_run, kLog2e, 15.0f));
-                l_run += p[i];
-            }
-            if (Q8) {
-                const int nb = d >> 5;
-                const __half* vsc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + 2 * kUnit * pitch + d);
-                // the largest value scale so far, rounded up to a power of two, is taken out of the weights (2^15 times it may
-                // pass f16's range) and kept beside the sums
-                float most = 0.0f;
-                for (int b = 0; b < nb; ++b)
+            for (int b = 0; b < NB; ++b) {
+                if (EXACT || b < nb) {
+                    uint32_t a[NT][2];  // leading parts and remainders of weight times scale
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) most = fmaxf(most, __half2float(vsc[(2 * t + (i & 1) + (i >> 1) * 8) * nb + b]));
-                if (__any_sync(0xffffffffu, most > v_bound)) {
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    const unsigned bits = (__float_as_uint(fminf(most, 65536.0f)) + 0x7fffffu) & 0xff800000u;
-                    const float bound = fmaxf(v_bound, __uint_as_float(bits)), r = v_bound / bound;
-                    v_bound = bound;
-                    v_factor = 1.0f / bound;
+                    for (int n = 0; n < NT; ++n) {
+                        __half2 s2 = half2_of(__byte_perm(w[2 * n][b / 2], w[2 * n + 1][b / 2], (b & 1) ? 0x7632 : 0x5410));
+                        if (!plain) s2 = __hmul2(s2, v_norm);
+                        const __half2 hi2 = __hmul2(half2_of(ph[n]), s2);
+                        const __half2 rest = __hfma2(half2_of(ph[n]), s2, __hneg2(hi2));
+                        a[n][0] = bits_of(hi2), a[n][1] = bits_of(__hfma2(half2_of(pl[n]), s2, rest));
+                    }
 #pragma unroll
-                    for (int n = 0; n < DM / 8; ++n) o[n][0] *= r, o[n][1] *= r, o[n][2] *= r, o[n][3] *= r;
-                }
-#pragma unroll
-                for (int b = 0; b < KS / 2; ++b) {
-                    if (b < nb) {
-                        uint32_t r[4], a[4];
-                        ldsm_x4_t(vs + v_lane + b * 32, r);  // values 0-15 of the block: keys 0-7, 8-15; values 16-31: the same
-                        const float w0 = p[0] * (__half2float(vsc[(2 * t) * nb + b]) * v_factor), w1 = p[1] * (__half2float(vsc[(2 * t + 1) * nb + b]) * v_factor);
-                        const float w2 = p[2] * (__half2float(vsc[(2 * t + 8) * nb + b]) * v_factor), w3 = p[3] * (__half2float(vsc[(2 * t + 9) * nb + b]) * v_factor);
-                        split2(w0, w1, a[0], a[1]);
-                        split2(w2, w3, a[2], a[3]);
+                    for (int n2 = 0; n2 < NT / 2; ++n2) {
+                        uint32_t r[4];
+                        const uint32_t aa[4] = {a[2 * n2][0], a[2 * n2][1], a[2 * n2 + 1][0], a[2 * n2 + 1][1]};
+                        ldsm_x4_t(vs + n2 * 16 * pitch + v_lane + b * 32, r);  // values 0-15 of the block: keys 0-7, 8-15; values 16-31: the same
 #pragma unroll
                         for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
                         // a lane's word: values 2g, 2g + 1 of key 2t, then of key 2t + 1
-                        mma16816(o[4 * b], a, widen<0x4240>(r[0]), widen<0x4240>(r[1]));
-                        mma16816(o[4 * b + 1], a, widen<0x4341>(r[0]), widen<0x4341>(r[1]));
-                        mma16816(o[4 * b + 2], a, widen<0x4240>(r[2]), widen<0x4240>(r[3]));
-                        mma16816(o[4 * b + 3], a, widen<0x4341>(r[2]), widen<0x4341>(r[3]));
+                        mma16816(o[4 * b], aa, widen<0x4240>(r[0]), widen<0x4240>(r[1]));
+                        mma16816(o[4 * b + 1], aa, widen<0x4341>(r[0]), widen<0x4341>(r[1]));
+                        mma16816(o[4 * b + 2], aa, widen<0x4240>(r[2]), widen<0x4240>(r[3]));
+                        mma16816(o[4 * b + 3], aa, widen<0x4341>(r[2]), widen<0x4341>(r[3]));
                     }
                 }
-            } else {
-                uint32_t a[4];
-                split2(p[0], p[1], a[0], a[1]);
-                split2(p[2], p[3], a[2], a[3]);
+            }
+        } else {
+#pragma unroll
+            for (int n2 = 0; n2 < NT / 2; ++n2) {
+                const uint32_t a[4] = {ph[2 * n2], pl[2 * n2], ph[2 * n2 + 1], pl[2 * n2 + 1]};
 #pragma unroll
                 for (int n = 0; n < KS; ++n) {
-                    if (n < steps) {
+                    if (EXACT || n < steps) {
                         uint32_t r[4];
-                        ldsm_x4_t(vs + v_lane + n * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
+                        ldsm_x4_t(vs + n2 * 16 * pitch + v_lane + n * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
                         mma16816(o[2 * n], a, r[0], r[1]);
                         mma16816(o[2 * n + 1], a, r[2], r[3]);
                     }
                 }
             }
         }
+        ring_sync();  // all the ring's warps are done with the values
+        copy_side(stage, 1);
+        step_ahead(stage);
         stage = stage + 1 == A.stages ? 0 : stage + 1;
 
         const bool ended = cur.u + 1 == cur.units;
         if (ended || done + 1 == count) {
-            const float l = [&] {
-                float x = l_run + __shfl_xor_sync(0xffffffffu, l_run, 1);
-                return x + __shfl_xor_sync(0xffffffffu, x, 2);
-            }();
+            l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+            l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
             const int row_id = cur.s * rows_per_seq + cur.r;
-            const float unit_v = Q8 ? v_bound : 1.0f;
-            const int in_row = part * A.heads_per_warp + g;
-            if (begin_u == 0 && ended) {
-                const int kvh = cur.r / A.passes, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
-                if (g < A.heads_per_warp && in_row < A.span && in_group < A.group) {
-                    const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
-                    const float inv = l > 0.0f || l != l ? unit_v / l : 0.0f;
-                    float* dst = A.out + at * d;
-#pragma unroll
-                    for (int n = 0; n < KS; ++n) {
-                        if (n < steps) {
-                            if (Q8) {
-                                *reinterpret_cast<float4*>(dst + 16 * n + 4 * t) =
-                                    make_float4(whole(o[2 * n][0], o[2 * n][2]) * inv, whole(o[2 * n + 1][0], o[2 * n + 1][2]) * inv,
-                                                whole(o[2 * n][1], o[2 * n][3]) * inv, whole(o[2 * n + 1][1], o[2 * n + 1][3]) * inv);
-                            } else {
-                                *reinterpret_cast<float2*>(dst + 16 * n + 2 * t) = make_float2(whole(o[2 * n][0], o[2 * n][2]) * inv, whole(o[2 * n][1], o[2 * n][3]) * inv);
-                                *reinterpret_cast<float2*>(dst + 16 * n + 8 + 2 * t) =
-                                    make_float2(whole(o[2 * n + 1][0], o[2 * n + 1][2]) * inv, whole(o[2 * n + 1][1], o[2 * n + 1][3]) * inv);
-                            }
-                        }
-                    }
-                    if (A.stats && t == 0) A.stats[at * 2] = l > 0.0f ? m_run : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
-                }
-            } else {
-                const int which = begin_u != 0 ? 0 : 1;
-                if (which == 1) ring_sync();  // the last piece of the share lands on the stages: all warps are done with them
-                float* pc = piece_ptr(ring, which) + (size_t)(part * kRowsPerWarp + g) * d;
-                float* ml = piece_ptr(ring, which) + (size_t)prow * d + (part * kRowsPerWarp + g) * 2;
+            const int in_row = part * A.heads_per_warp + g, kvh = cur.r / A.passes, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
+            const bool finished = begin_u == 0 && ended;
+            const bool live = g < A.heads_per_warp && in_row < A.span && in_group < A.group;
+            const int which = begin_u != 0 ? 0 : 1;
+            const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
+            // a piece on the stages is the share's last: all warps are done with them
+            if (!finished && (which == 1 || A.row_mode)) ring_sync();
+            float* pc = piece_ptr(ring, which);
+            float* dst = finished ? A.out + at * d : pc + (size_t)(part * kRowsPerWarp + g) * d;
+            const float f = finished ? (l_run > 0.0f || l_run != l_run ? v_unit / l_run : 0.0f) : v_unit;
+            if (live || !finished) {
 #pragma unroll
                 for (int n = 0; n < KS; ++n) {
-                    if (n < steps) {
+                    if (EXACT || n < steps) {
+                        const float a = whole(o[2 * n][0], o[2 * n][2]) * f, b = whole(o[2 * n][1], o[2 * n][3]) * f;
+                        const float c = whole(o[2 * n + 1][0], o[2 * n + 1][2]) * f, e = whole(o[2 * n + 1][1], o[2 * n + 1][3]) * f;
                         if (Q8) {
-                            float* x = pc + 16 * n + 4 * t;
-                            x[0] = whole(o[2 * n][0], o[2 * n][2]) * unit_v, x[1] = whole(o[2 * n + 1][0], o[2 * n + 1][2]) * unit_v;
-                            x[2] = whole(o[2 * n][1], o[2 * n][3]) * unit_v, x[3] = whole(o[2 * n + 1][1], o[2 * n + 1][3]) * unit_v;
+                            *reinterpret_cast<float4*>(dst + 16 * n + 4 * t) = make_float4(a, c, b, e);
                         } else {
-                            float* x = pc + 16 * n + 2 * t;
-                            x[0] = whole(o[2 * n][0], o[2 * n][2]), x[1] = whole(o[2 * n][1], o[2 * n][3]);
-                            x[8] = whole(o[2 * n + 1][0], o[2 * n + 1][2]), x[9] = whole(o[2 * n + 1][1], o[2 * n + 1][3]);
+                            *reinterpret_cast<float2*>(dst + 16 * n + 2 * t) = make_float2(a, b);
+                            *reinterpret_cast<float2*>(dst + 16 * n + 8 + 2 * t) = make_float2(c, e);
                         }
                     }
                 }
-                if (t == 0) ml[0] = m_run, ml[1] = l;
+            }
+            if (finished) {
+                if (A.stats && live && t == 0) A.stats[at * 2] = l_run > 0.0f ? m_run : kNegBig, A.stats[at * 2 + 1] = l_run * (1.0f / 32768.0f);
+            } else {
+                float* ml = pc + (size_t)prow * d + (part * kRowsPerWarp + g) * 2;
+                if (t == 0) ml[0] = m_run, ml[1] = l_run;
                 const long long last_unit = from + done + (cur.units - 1 - cur.u);
                 if (part == 0 && lane == 0) sh_piece[ring][which] = {row_id, ended ? -1 : (int)(last_unit / share / A.rings)};
             }
@@ -523,53 +629,61 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) attn_paged_kernel(const Pag
         cur.next(A, rows_per_seq);
     }
 
-    // ---- join the pieces inside the CTA, in order; what still lacks its beginning or its end goes to the workspace
+    // ---- join the pieces inside the CTA, in order (a warp per head row, a lane per piece for the weights, then four values a
+    // lane); what still lacks its beginning or its end goes to the workspace
     __syncthreads();
-    const int entries = 2 * A.rings;
-    auto entry = [&](int e) { return sh_piece[e >> 1][e & 1]; };
+    const int entries = 2 * A.rings, warps = blockDim.x >> 5;
+    Piece mine{-1, -1};
+    if (lane < entries) mine = sh_piece[lane >> 1][lane & 1];
     int tail_row = -1, tail_last = 0;
-    for (int e0 = 0; e0 < entries;) {
-        const Piece p0 = entry(e0);
-        if (p0.row < 0) {
-            ++e0;
-            continue;
-        }
-        int e1 = e0 + 1;
-        bool ended = p0.last < 0;
-        while (e1 < entries && (entry(e1).row < 0 || entry(e1).row == p0.row)) {
-            if (entry(e1).row == p0.row) ended = entry(e1).last < 0;
-            ++e1;
-        }
-        const bool begun = (e0 & 1) != 0;
-        const int s = p0.row / rows_per_seq, r = p0.row - s * rows_per_seq, kvh = r / A.passes;
-        if (begun && !ended) tail_row = p0.row, tail_last = p0.last;
-        for (int i = threadIdx.x; i < prow * d; i += blockDim.x) {
-            const int pr = i / d, dim = i - pr * d;
-            float m = -INFINITY, l = 0.0f, a = 0.0f;
-            for (int e = e0; e < e1; ++e)
-                if (entry(e).row == p0.row) m = fmaxf(m, piece_ptr(e >> 1, e & 1)[(size_t)prow * d + pr * 2]);
-            for (int e = e0; e < e1; ++e)
-                if (entry(e).row == p0.row) {
-                    const float* pc = piece_ptr(e >> 1, e & 1);
-                    const float pm = pc[(size_t)prow * d + pr * 2];
-                    const float f = pm == -INFINITY ? 0.0f : ex2((pm - m) * kLog2e);
-                    l += pc[(size_t)prow * d + pr * 2 + 1] * f;
-                    a += pc[(size_t)pr * d + dim] * f;
+    for (unsigned todo = __ballot_sync(0xffffffffu, mine.row >= 0); todo;) {
+        const int e0 = __ffs(todo) - 1;
+        const int row = __shfl_sync(0xffffffffu, mine.row, e0);
+        const unsigned run = __ballot_sync(0xffffffffu, mine.row == row);
+        const int e1 = 31 - __clz(run);
+        const bool begun = (e0 & 1) != 0, ended = __shfl_sync(0xffffffffu, mine.last, e1) < 0;
+        if (begun && !ended) tail_row = row, tail_last = __shfl_sync(0xffffffffu, mine.last, e0);
+        const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
+        for (int pr = warp; pr < prow; pr += warps) {
+            float m = -INFINITY, l = 0.0f;
+            const bool in = (run >> lane) & 1;
+            if (in) {
+                const float* ml = piece_ptr(lane >> 1, lane & 1) + (size_t)prow * d + pr * 2;
+                m = ml[0], l = ml[1];
+            }
+            float m_all = m;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
+            const float f = m == -INFINITY ? 0.0f : ex2((m - m_all) * kLog2e);
+            l *= f;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
+            const bool live = (pr & 7) < A.heads_per_warp && in_row < A.span && in_group < A.group;
+            const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
+            const bool finished = begun && ended;
+            float* part_out = A.parts + ((size_t)blockIdx.x * (2 + A.rings) + (begun ? 1 : 0)) * piece_floats;
+            float* dst = finished ? A.out + at * d : part_out + (size_t)pr * d;
+            const float inv = !finished ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            for (int i0 = 0; i0 < d; i0 += 128) {
+                const int i = i0 + lane * 4;
+                float4 a = make_float4(0, 0, 0, 0);
+                for (unsigned rest = run; rest; rest &= rest - 1) {
+                    const int e = __ffs(rest) - 1;
+                    const float fe = __shfl_sync(0xffffffffu, f, e);
+                    if (i < d) {
+                        const float4 x = *reinterpret_cast<const float4*>(piece_ptr(e >> 1, e & 1) + (size_t)pr * d + i);
+                        a.x = fmaf(x.x, fe, a.x), a.y = fmaf(x.y, fe, a.y), a.z = fmaf(x.z, fe, a.z), a.w = fmaf(x.w, fe, a.w);
+                    }
                 }
-            if (begun && ended) {
-                const int wp = pr >> 3, in_row = wp * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
-                if ((pr & 7) < A.heads_per_warp && in_row < A.span && in_group < A.group) {
-                    const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
-                    A.out[at * d + dim] = l > 0.0f || l != l ? a / l : 0.0f;
-                    if (A.stats && dim == 0) A.stats[at * 2] = l > 0.0f ? m : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
-                }
-            } else {
-                float* dst = A.parts + ((size_t)blockIdx.x * 2 + (begun ? 1 : 0)) * piece_floats;
-                dst[(size_t)pr * d + dim] = a;
-                if (dim == 0) dst[(size_t)prow * d + pr * 2] = m, dst[(size_t)prow * d + pr * 2 + 1] = l;
+                if (i < d && (live || !finished)) *reinterpret_cast<float4*>(dst + i) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            }
+            if (lane == 0) {
+                if (!finished) part_out[(size_t)prow * d + pr * 2] = m_all, part_out[(size_t)prow * d + pr * 2 + 1] = l;
+                else if (A.stats && live) A.stats[at * 2] = l > 0.0f ? m_all : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
             }
         }
-        e0 = e1;
+        todo &= ~run;
     }
     if (!A.row_mode && threadIdx.x == 0) A.meta[blockIdx.x * 2] = tail_row, A.meta[blockIdx.x * 2 + 1] = tail_last;
 }
@@ -590,7 +704,7 @@ __global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedArgs A)
     const int prow = A.warps_per_ring * kRowsPerWarp, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t piece_floats = (size_t)prow * (d + 2);
     const int n = A.meta[c0 * 2 + 1] - c0 + 1;
-    auto piece = [&](int i) { return A.parts + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats; };
+    auto piece = [&](int i) { return A.parts + ((size_t)(c0 + i) * (2 + A.rings) + (i == 0 ? 1 : 0)) * piece_floats; };
     float m = -INFINITY;
     for (int i = threadIdx.x; i < n; i += 128) m = fmaxf(m, piece(i)[(size_t)prow * d + pr * 2]);
 #pragma unroll
@@ -627,9 +741,9 @@ __global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedArgs A)
 
 // How a call is cut, from sizes the host knows.
 struct Plan {
-    int passes, span, warps_per_ring, heads_per_warp, rings, stages, stage_bytes;
+    int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stages, stage_bytes;
     int row_mode, grid;
-    size_t smem, piece_floats, workspace;
+    size_t smem, workspace;
 };
 
 // At least two units of a row per share: below that the joins cost more than the copies they spread.
@@ -638,46 +752,47 @@ constexpr int kMinUnits = 2;
 int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max_len, int sm_count, Plan* out) {
     Plan p;
     const int group = (int)heads / c.kv_heads, d = c.d;
+    p.exact = d == 64 || d == 128 || d == 256;
+    p.dm = d <= 64 && p.exact ? 64 : d <= 128 ? 128 : 256;
     p.passes = (group + 31) / 32;
     p.span = (group + p.passes - 1) / p.passes;
     p.warps_per_ring = (p.span + kRowsPerWarp - 1) / kRowsPerWarp;
     p.heads_per_warp = (p.span + p.warps_per_ring - 1) / p.warps_per_ring;
-    const int pitch = ((q8 ? d / 16 : d / 8) + 1) * 16, unit_bytes = kUnit * d * (q8 ? 2 : 4);
-    p.stage_bytes = 2 * kUnit * pitch + (q8 ? 2 * d : 0);
-    const int piece = p.warps_per_ring * kRowsPerWarp * (d + 2) * (int)sizeof(float);
-    // the most rings that still leave 96 KB of copies in flight, else the most bytes in flight
-    int best = -1;
-    p.rings = p.stages = 0;
-    for (int rings = kMaxWarps / p.warps_per_ring; rings >= 1; --rings) {
-        int stages = (kSmemMost / rings - piece) / p.stage_bytes;
-        stages = stages > kMaxStages ? kMaxStages : stages;
-        if (stages < 2 || stages * p.stage_bytes < piece) continue;
-        const int flying = rings * (stages - 1) * unit_bytes;
-        if (flying > best) best = flying, p.rings = rings, p.stages = stages;
-        if (flying >= 96 * 1024) break;
-    }
-    if (best < 0) return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
-    p.smem = (size_t)p.rings * ((size_t)p.stages * p.stage_bytes + piece);
-    p.piece_floats = piece / sizeof(float);
-    const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / kUnit + 2;
+    const int keys = unit_keys(p.dm), pitch = ((q8 ? d / 16 : d / 8) + 1) * 16;
+    p.stage_bytes = 2 * keys * pitch + (q8 ? 4 * keys * (d / 32) : 0);
+    const size_t piece = (size_t)p.warps_per_ring * kRowsPerWarp * (d + 2) * sizeof(float);
+    // as many rings as warps and two stages each allow; a third stage where there is room
+    p.rings = max_warps(p.dm) / p.warps_per_ring;
+    while (p.rings > 1 && p.rings * 2 * p.stage_bytes > kSmemMost) --p.rings;
+    p.stages = p.rings * 3 * p.stage_bytes <= kSmemMost ? 3 : 2;
+    if (p.rings * p.stages * p.stage_bytes > kSmemMost || (size_t)p.stages * p.stage_bytes < piece)
+        return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
+    p.smem = (size_t)p.rings * p.stages * p.stage_bytes;
+    const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / keys + 2;
     if (rows > (size_t)INT32_MAX / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
-    p.row_mode = units <= (size_t)8 * p.rings;
+    p.row_mode = units <= (size_t)4 * p.rings;
     const size_t shares = (rows * units + kMinUnits - 1) / kMinUnits, ctas = (shares + p.rings - 1) / p.rings;
     p.grid = p.row_mode ? (int)rows : (int)(ctas < (size_t)sm_count ? ctas : (size_t)sm_count);
-    p.workspace = p.row_mode ? 0 : (size_t)p.grid * 16 + (size_t)p.grid * 2 * p.piece_floats * sizeof(float);
+    p.workspace = p.row_mode ? 0 : (size_t)p.grid * (16 + (2 + p.rings) * piece);
     *out = p;
     return FQ_OK;
 }
 
-template <bool Q8, int DM>
+template <bool Q8, int DM, bool EXACT>
 cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
     static bool granted = false;  // under the dispatch lock
     if (!granted) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<Q8, DM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<Q8, DM, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
         if (e != cudaSuccess) return e;
         granted = true;
     }
-    return launch_pdl(attn_paged_kernel<Q8, DM>, dim3((unsigned)p.grid), dim3((unsigned)(p.rings * p.warps_per_ring * 32)), p.smem, st, a);
+    return launch_pdl(attn_paged_kernel<Q8, DM, EXACT>, dim3((unsigned)p.grid), dim3((unsigned)(p.rings * p.warps_per_ring * 32)), p.smem, st, a);
+}
+template <bool Q8>
+cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
+    if (p.dm == 64) return launch_paged<Q8, 64, true>(a, p, st);
+    if (p.dm == 128) return p.exact ? launch_paged<Q8, 128, true>(a, p, st) : launch_paged<Q8, 128, false>(a, p, st);
+    return p.exact ? launch_paged<Q8, 256, true>(a, p, st) : launch_paged<Q8, 256, false>(a, p, st);
 }
 
 int check_paged(const fq_kv_pages* pages, size_t n_seqs, size_t heads, KvView* c) {
@@ -751,12 +866,10 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
     a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp;
     a.rings = p.rings, a.stages = p.stages, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.min_units = kMinUnits;
-    const unsigned long long per_page = (unsigned long long)(c.page_tokens / kUnit);
-    a.page_magic = ((1ull << 32) + per_page - 1) / per_page;  // exact below 2^32 / 256 units
+    const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
+    a.page_magic = ((1ull << 32) + per_page - 1) / per_page;  // exact below 2^32 / 256 times 16 keys
     a.meta = (int*)ws, a.parts = (float*)(ws + (size_t)p.grid * 16);
-    cudaError_t e;
-    if (q8) e = c.d <= 64 ? launch_paged<true, 64>(a, p, st) : c.d <= 128 ? launch_paged<true, 128>(a, p, st) : launch_paged<true, 256>(a, p, st);
-    else e = c.d <= 64 ? launch_paged<false, 64>(a, p, st) : c.d <= 128 ? launch_paged<false, 128>(a, p, st) : launch_paged<false, 256>(a, p, st);
+    cudaError_t e = q8 ? launch_paged<true>(a, p, st) : launch_paged<false>(a, p, st);
     g_trace.launches++;
     if (e == cudaSuccess && !p.row_mode) {
         e = launch_pdl(attn_paged_join_kernel, dim3((unsigned)p.grid, (unsigned)(p.warps_per_ring * kRowsPerWarp)), dim3(128), 0, st, a);

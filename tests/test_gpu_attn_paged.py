@@ -166,6 +166,24 @@ def test_shared_prefix_pages(P):
 
 
 @pytest.mark.parametrize("kind", ["f16", "q8_0"])
+@pytest.mark.parametrize("window", [1, 15, 16, 17, 31, 32, 33, 100])
+def test_pages_behind_the_window_may_be_gone(P, kind, window):
+    """A sliding window's user hands pages that lie wholly before the window to other sequences."""
+    import torch
+
+    rng = np.random.default_rng(23)
+    lens = [130, 129, 145, 4000]
+    cache = Cache(P, kind, lens, 16, 1, 64, rng)
+    rows = cache.fill(rng)
+    for s, n in enumerate(lens):
+        cache.table[s, : (n - window) // 16] = -1
+    torch.cuda.synchronize()
+    q = rng.standard_normal((len(lens), 3, 64)).astype(np.float32)
+    got, _ = cache.attend(q, 3, 0.125, window)
+    check_attention(cache, rows, q, got, 0.125, window)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
 @pytest.mark.parametrize("lens", [[500], [9000], [3000, 200, 6000]])
 def test_bad_pages_and_lengths_are_reported_and_left_out(P, kind, lens):
     import torch
