@@ -10,7 +10,7 @@
 //
 // Split. Work is counted in units of 32 keys (16 where a row of K is longer than 128 values) of one kv head; a row is one
 // (sequence, kv head). All units of all rows, in order, are cut into equal shares, one per ring: uneven lengths load the
-// GPU evenly and one long sequence uses all of it. A ring is two or three shared-memory stages of one unit each, filled by
+// GPU evenly and one long sequence uses all of it. A ring is two shared-memory stages of one unit each, filled by
 // cp.async and walked by 1 to 4 warps, each with up to eight of the query heads that share the kv head. A row that lies
 // inside one ring's share is finished there; pieces of rows that cross shares are joined inside the CTA, and pieces that
 // cross CTAs go to the workspace and are joined, in order, by a second kernel. When every row is short, one CTA takes one
@@ -62,11 +62,12 @@ struct PagedArgs {
     int* status;
     int passes;        // a kv head with more than 32 query heads is walked in this many rows of `span` heads
     int span;          // query heads of one row
-    int warps_per_ring, heads_per_warp, rings, stages;
+    int warps_per_ring, heads_per_warp, rings;
     int stage_bytes;
     int row_mode;      // one CTA per row; else shares of at least min_units
     int min_units;
-    unsigned long long page_magic;  // (16 keys) / (16 keys of a page) = x * page_magic >> 32
+    unsigned page_magic;                  // index of 16 keys / 16-key runs of a page = umulhi(index, page_magic); 0: one run a page
+    unsigned page_chunks, scale_chunks;   // 16-byte chunks from page to page
     int* meta;         // [grid][2]: the row whose beginning CTA c holds in part 1 (-1: none), the last CTA with a piece of it (in part 0)
     float* parts;      // [grid][2 + rings][warps_per_ring * 8][d + 2]: o, then max and sum; part 2 + r: the first piece of ring r
 };
@@ -75,11 +76,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// the oldest of the 2 * stages groups under way has landed
-__device__ __forceinline__ void cp_async_wait_oldest(int stages) {
-    if (stages == 2) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else asm volatile("cp.async.wait_group 5;" ::: "memory");
-}
+// the oldest of the four groups under way has landed
+__device__ __forceinline__ void cp_async_wait_oldest() { asm volatile("cp.async.wait_group 3;" ::: "memory"); }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -138,20 +136,22 @@ __device__ __forceinline__ int units_of(int first, int end) {
     return max(1, (end + UK - 1) / UK - first / UK);
 }
 
-// Where a ring stands: unit `u` of row `r` of sequence `s`.
+// Where a ring stands: `left` units of row `r` of sequence `s` are to come, from the keys `key` on.
 template <int UK>
 struct Cursor {
-    int s, r, u, units, first, end;
-    __device__ __forceinline__ void load(const PagedArgs& A) {
-        key_range(A, s, first, end);
-        units = units_of<UK>(first, end);
-    }
-    __device__ __forceinline__ void next(const PagedArgs& A, int rows_per_seq) {
-        if (++u < units) return;
-        u = 0;
-        if (++r < rows_per_seq) return;
-        r = 0;
-        if (++s < A.n_seqs) load(A);
+    int s, r, left, key, first, end;
+    __device__ __forceinline__ int units() const { return units_of<UK>(first, end); }
+    __device__ __forceinline__ void start_row(int u) { left = units() - u, key = (first / UK + u) * UK; }
+    // past a unit; true when that entered another row
+    __device__ __forceinline__ bool next(const PagedArgs& A, int rows_per_seq) {
+        key += UK;
+        if (--left > 0) return false;
+        if (++r == rows_per_seq) {
+            r = 0;
+            if (++s < A.n_seqs) key_range(A, s, first, end);
+        }
+        start_row(0);
+        return true;
     }
 };
 
@@ -199,11 +199,11 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     const int piece_floats = prow * (d + 2);
     // a stage: K rows, V rows, and for Q8_0 their scales [UK][d / 32]
     const int k_scale_at = 2 * UK * pitch, v_scale_at = k_scale_at + UK * 2 * nb;
-    uint8_t* ring_base = smem + (size_t)ring * A.stages * A.stage_bytes;
+    uint8_t* ring_base = smem + (size_t)ring * 2 * A.stage_bytes;
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring_base);
     auto piece_ptr = [&](int rg, int which) {
         return which == 0 && !A.row_mode ? A.parts + ((size_t)blockIdx.x * (2 + A.rings) + 2 + rg) * piece_floats
-                                         : reinterpret_cast<float*>(smem + (size_t)rg * A.stages * A.stage_bytes);
+                                         : reinterpret_cast<float*>(smem + (size_t)rg * 2 * A.stage_bytes);
     };
 
     // ---- this ring's share
@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     long long from = 0;
     if (A.row_mode) {
         cur.s = blockIdx.x / rows_per_seq, cur.r = blockIdx.x - cur.s * rows_per_seq;
-        cur.load(A);
-        cur.u = (int)((long long)cur.units * ring / A.rings);
-        count = (int)((long long)cur.units * (ring + 1) / A.rings) - cur.u;
+        key_range(A, cur.s, cur.first, cur.end);
+        const int units = cur.units(), u = units * ring / A.rings;  // a row of few units
+        count = units * (ring + 1) / A.rings - u;
+        cur.start_row(u);
     } else {
         int mine = 0;
         for (int s = lane; s < A.n_seqs; s += 32) {
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         share = max(A.min_units, (int)(((long long)total + workers - 1) / workers));
         from = (long long)(blockIdx.x * A.rings + ring) * share;
         count = (int)max(0ll, min((long long)share, total - from));
-        cur.s = cur.r = cur.u = 0, cur.units = 1, cur.first = cur.end = 0;
+        cur = {0, 0, 1, 0, 0, 0};
         if (count > 0) {
             // the sequence that holds unit `from`
             int before = 0;
@@ -246,8 +247,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                     const int local = (int)(from - before) - __shfl_sync(0xffffffffu, sum - n, l);
                     cur.s = s0 + l;
                     cur.first = __shfl_sync(0xffffffffu, first, l), cur.end = __shfl_sync(0xffffffffu, end, l);
-                    cur.units = units_of<UK>(cur.first, cur.end);
-                    cur.r = local / cur.units, cur.u = local - cur.r * cur.units;
+                    cur.r = local / cur.units();
+                    cur.start_row(local - cur.r * cur.units());
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
@@ -256,87 +257,99 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     }
     if (part == 0 && lane < 2) sh_piece[ring][lane] = {-1, -1};
 
-    // ---- copies. `ahead` is the unit copied next, `tok[x]` the place of its x-th 16 keys (tokens of all pages and heads in
-    // storage order; -1: nothing to copy), looked up one step before it is needed. `gone`: per stage and 16 keys, a bit for
-    // keys whose page is no page.
+    // ---- copies. `ahead` is the unit copied next; its pages are looked up a step before they are needed. A unit is one or two
+    // runs of 16 keys, each inside one page: run x starts `run[x]` chunks into k and v (its scales `srun[x]` chunks into theirs).
+    constexpr int RUNS = UK / kSub;
     Cursor<UK> ahead = cur;
     int left = count;
-    unsigned gone = 0, gone_next = 0;
-    int pg[UK / kSub], pu[UK / kSub];
-    const int subs_per_page = A.c.page_tokens / kSub;
+    unsigned have = 0;  // runs of the unit to copy that exist
+    unsigned gone_new = 0, gone_next = 0, gone_now = 0;  // runs whose page is no page: of the unit to copy, and of the two in the stages
+    int pg[RUNS], pu[RUNS];
+    size_t run[RUNS], srun[RUNS];
+    const int runs_per_page = A.c.page_tokens / kSub;
+    const int* table = A.table;
+    int head_run = 0;
+    auto enter_row = [&]() {
+        table = A.table + (size_t)ahead.s * A.max_pages;
+        head_run = ahead.r / A.passes * runs_per_page;
+    };
     auto look_up = [&]() {
-        gone_next = 0;
 #pragma unroll
-        for (int x = 0; x < UK / kSub; ++x) {
-            const int sub = (ahead.first / UK + ahead.u) * (UK / kSub) + x;
+        for (int x = 0; x < RUNS; ++x) {
+            const int i = ahead.key / kSub + x;
             pg[x] = -1;
-            if (sub * kSub < ahead.end && (sub + 1) * kSub > ahead.first) {
-                const int slot = (int)(((unsigned long long)(unsigned)sub * A.page_magic) >> 32);
-                pu[x] = sub - slot * subs_per_page;
-                pg[x] = A.table[(size_t)ahead.s * A.max_pages + slot];
+            if (i * kSub < ahead.end && (i + 1) * kSub > ahead.first) {
+                const int slot = A.page_magic ? (int)__umulhi((unsigned)i, A.page_magic) : i;
+                pu[x] = head_run + i - slot * runs_per_page;
+                pg[x] = table[slot];
             }
         }
     };
-    // (after the loads have arrived) which of them name no page
-    auto judge = [&]() {
+    // after the look-up's loads have arrived
+    auto place = [&]() {
+        have = gone_new = 0;
 #pragma unroll
-        for (int x = 0; x < UK / kSub; ++x) {
-            const int sub = (ahead.first / UK + ahead.u) * (UK / kSub) + x;
-            if (sub * kSub < ahead.end && (sub + 1) * kSub > ahead.first && (pg[x] < 0 || pg[x] >= A.c.n_pages)) {
+        for (int x = 0; x < RUNS; ++x) {
+            const int i = ahead.key / kSub + x;
+            if ((unsigned)pg[x] < (unsigned)A.c.n_pages) {
+                have |= 1u << x;
+                run[x] = (size_t)(unsigned)pg[x] * A.page_chunks + (unsigned)(pu[x] * kSub * nc);
+                if (Q8) srun[x] = (size_t)(unsigned)pg[x] * A.scale_chunks + (unsigned)(pu[x] * nc);
+            } else if (i * kSub < ahead.end && (i + 1) * kSub > ahead.first) {
                 *(volatile int*)A.status = FQ_ERR_PAGE;
-                gone_next |= 1u << x;
-                pg[x] = -1;
+                gone_new |= 1u << x;
             }
         }
     };
     const unsigned row_magic = (65536u + nc - 1) / nc;  // chunk / nc = chunk * row_magic >> 16 for chunks < 512
-    // the keys (side 0) or values of the unit at `ahead` into `stage`
-    auto copy_side = [&](int stage, int side) {
+    const uint32_t copy_dst = ring_addr + (EXACT ? (lane + lane / nc) * 16 : 0);
+    const uint8_t* const copy_k = A.c.k + lane * 16;
+    const uint8_t* const copy_v = A.c.v + lane * 16;
+    // the keys (side 0) or values of the unit to copy into the stage at `stage_at`; the ring's warps take every n-th instruction
+    auto copy_side = [&](uint32_t stage_at, int side) {
         if (left > 0) {
 #pragma unroll
-            for (int x = 0; x < UK / kSub; ++x) {
-                if (pg[x] >= 0) {
-                    const size_t tok = (size_t)(ahead.r / A.passes) * A.c.page_tokens + (size_t)pu[x] * kSub;
-                    const size_t off = ((size_t)pg[x] * A.c.page_stride + tok * d) * (Q8 ? 1 : 2);
-                    const uint8_t* src = (side ? A.c.v : A.c.k) + off + lane * 16;
-                    const uint32_t base = ring_addr + stage * A.stage_bytes + (side * UK + x * kSub) * pitch;
-                    if (EXACT) {
-                        // 32 / nc or nc / 32 rows at a time
-                        const uint32_t dst = base + (lane + lane / nc) * 16;
+            for (int x = 0; x < RUNS; ++x) {
+                if ((have >> x) & 1) {
+                    const uint8_t* src = (side ? copy_v : copy_k) + run[x] * 16;
+                    const uint32_t dst = copy_dst + stage_at + (side * UK + x * kSub) * pitch;
+                    if (EXACT && A.warps_per_ring == 1) {
+#pragma unroll
+                        for (int i = 0; i < (Q8 ? DM / 32 : DM / 16); ++i) cp_async16(dst + i * (512 + 512 / nc), src + i * 512);
+                    } else if (EXACT) {
                         for (int i = part; i < nc / 2; i += A.warps_per_ring) cp_async16(dst + i * (512 + 512 / nc), src + i * 512);
                     } else {
                         for (int i = part; i < nc / 2; i += A.warps_per_ring) {
                             const int c = lane + 32 * i, row = (int)((c * row_magic) >> 16);
-                            cp_async16(base + (c + row) * 16, src + i * 512);
+                            cp_async16(dst + (c + row) * 16, src + i * 512);
                         }
                     }
-                    if (Q8 && part == 0 && lane < nc) {  // 16 keys x d / 32 scales = d bytes
-                        const size_t so = (size_t)pg[x] * A.c.scale_stride + tok * nb;
-                        cp_async16(ring_addr + stage * A.stage_bytes + (side ? v_scale_at : k_scale_at) + x * d + lane * 16,
-                                   reinterpret_cast<const uint8_t*>((side ? A.c.v_scale : A.c.k_scale) + so) + lane * 16);
-                    }
+                    if (Q8 && part == 0 && lane < nc)  // 16 keys x d / 32 scales = d bytes
+                        cp_async16(ring_addr + stage_at + (side ? v_scale_at : k_scale_at) + x * d + lane * 16,
+                                   reinterpret_cast<const uint8_t*>(side ? A.c.v_scale : A.c.k_scale) + srun[x] * 16 + lane * 16);
                 }
             }
         }
         cp_async_commit();
     };
-    auto step_ahead = [&](int stage) {
-        gone = (gone & ~(3u << (2 * stage))) | gone_next << (2 * stage);
-        if (left > 0) {
-            ahead.next(A, rows_per_seq);
-            if (--left > 0) look_up();
+    auto step_ahead = [&]() {
+        gone_now = gone_next, gone_next = gone_new;
+        if (--left > 0) {
+            if (ahead.next(A, rows_per_seq)) enter_row();
+            look_up();
         }
     };
     auto ring_sync = [&]() {
         if (A.warps_per_ring == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(ring + 1), "r"(A.warps_per_ring * 32) : "memory");
     };
-    if (count > 0) look_up();
-    for (int s = 0; s < A.stages; ++s) {
-        if (left > 0) judge();
-        copy_side(s, 0);
-        copy_side(s, 1);
-        step_ahead(s);
+    if (count > 0) enter_row(), look_up();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (left > 0) place();
+        copy_side(s * A.stage_bytes, 0);
+        copy_side(s * A.stage_bytes, 1);
+        step_ahead();
     }
 
     // ---- the share, piece by piece
@@ -344,8 +357,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     float o[DM / 8][4], l_run = 0.0f, m_run = -INFINITY, m_use = 0.0f, row_scale = 1.0f;
     float v_cap = 0.0f, v_unit = 1.0f;  // Q8_0: value scales up to v_cap so far; sums count in multiples of v_unit (a power of two)
     __half2 v_norm = half2_of(0x3c003c00u);  // 1 / v_unit
-    bool started = false;
-    int begin_u = 0, stage = 0;
+    bool started = false, begun_here = false;
+    uint32_t stage_at = 0;
     const int mi = lane >> 3, mr = lane & 7;
     const uint32_t k_lane = (uint32_t)(((mi >> 1) * 8 + mr) * pitch + (mi & 1) * 16);
     const uint32_t v_lane = (uint32_t)(((mi & 1) * 8 + mr) * pitch + (mi >> 1) * 16);
@@ -353,7 +366,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     for (int done = 0; done < count; ++done) {
         if (!started) {
             started = true;
-            begin_u = cur.u;
+            begun_here = cur.key == cur.first / UK * UK;
             // query fragments: row g = head g of this warp, times a power of two that puts the row's largest value near 2^14
             const int kvh = cur.r / A.passes, pass = cur.r - kvh * A.passes;
             const int in_row = part * A.heads_per_warp + g, in_group = pass * A.span + in_row;
@@ -397,19 +410,18 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
 #pragma unroll
             for (int n = 0; n < DM / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         }
-        const int j0 = (cur.first / UK + cur.u) * UK;
-        const int lo = max(cur.first - j0, 0), hi = min(cur.end - j0, UK);
-        const unsigned lost = (gone >> (2 * stage)) & 3;
+        const int lo = max(cur.first - cur.key, 0), hi = min(cur.end - cur.key, UK);
+        const unsigned lost = gone_now;
         const bool partial = hi - lo < UK || lost;  // some keys do not take part
-        const uint32_t ks = ring_addr + stage * A.stage_bytes, vs = ks + UK * pitch;
+        const uint32_t ks = ring_addr + stage_at, vs = ks + UK * pitch;
         auto takes_part = [&](int key) { return key >= lo && key < hi && !((lost >> (key / kSub)) & 1); };
 
         // ---- scores: keys 8 n + 2t, + 1 for head g
-        cp_async_wait_oldest(A.stages);
+        cp_async_wait_oldest();
         ring_sync();  // the keys' copies of all the ring's warps have landed
         float sc[NT][2];
         if (Q8) {
-            const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + k_scale_at);
+            const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage_at + k_scale_at);
 #pragma unroll
             for (int n2 = 0; n2 < NT / 2; ++n2) {  // sixteen keys at a time
                 uint32_t w[4][(NB + 1) / 2];
@@ -462,8 +474,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             for (int n = 0; n < NT; ++n) sc[n][0] = whole(c[n][0], c[n][2]), sc[n][1] = whole(c[n][1], c[n][3]);
         }
         ring_sync();  // all the ring's warps are done with the keys
-        if (left > 0) judge();
-        copy_side(stage, 0);
+        if (left > 0) place();
+        copy_side(stage_at, 0);
 
         // ---- weights
         float top = -INFINITY;
@@ -497,12 +509,12 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         }
 
         // ---- values
-        cp_async_wait_oldest(A.stages);
+        cp_async_wait_oldest();
         ring_sync();  // the values' copies have landed
         if (partial) {
             // values that do not take part may be anything: their rows (Q8_0: their scales) become zeros. The ring's warps write
             // the same zeros.
-            uint8_t* rows = ring_base + stage * A.stage_bytes + (Q8 ? v_scale_at : UK * pitch);
+            uint8_t* rows = ring_base + stage_at + (Q8 ? v_scale_at : UK * pitch);
             const int bytes = Q8 ? nb * 2 : d * 2, step = Q8 ? nb * 2 : pitch;
             for (int r = 0; r < UK; ++r)
                 if (!takes_part(r))
@@ -510,7 +522,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             __syncwarp();
         }
         if (Q8) {
-            const __half* vsc = reinterpret_cast<const __half*>(ring_base + stage * A.stage_bytes + v_scale_at);
+            const __half* vsc = reinterpret_cast<const __half*>(ring_base + stage_at + v_scale_at);
             uint32_t w[2 * NT][(NB + 1) / 2];
 #pragma unroll
             for (int i = 0; i < 2 * NT; ++i) load_scales<NB, EXACT>(vsc + (8 * (i >> 1) + 2 * t + (i & 1)) * nb, nb, w[i]);
@@ -582,19 +594,19 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             }
         }
         ring_sync();  // all the ring's warps are done with the values
-        copy_side(stage, 1);
-        step_ahead(stage);
-        stage = stage + 1 == A.stages ? 0 : stage + 1;
+        copy_side(stage_at, 1);
+        step_ahead();
+        stage_at = A.stage_bytes - stage_at;
 
-        const bool ended = cur.u + 1 == cur.units;
+        const bool ended = cur.left == 1;
         if (ended || done + 1 == count) {
             l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
             l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
             const int row_id = cur.s * rows_per_seq + cur.r;
             const int in_row = part * A.heads_per_warp + g, kvh = cur.r / A.passes, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
-            const bool finished = begin_u == 0 && ended;
+            const bool finished = begun_here && ended;
             const bool live = g < A.heads_per_warp && in_row < A.span && in_group < A.group;
-            const int which = begin_u != 0 ? 0 : 1;
+            const int which = begun_here ? 1 : 0;
             const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
             // a piece on the stages is the share's last: all warps are done with them
             if (!finished && (which == 1 || A.row_mode)) ring_sync();
@@ -621,7 +633,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             } else {
                 float* ml = pc + (size_t)prow * d + (part * kRowsPerWarp + g) * 2;
                 if (t == 0) ml[0] = m_run, ml[1] = l_run;
-                const long long last_unit = from + done + (cur.units - 1 - cur.u);
+                const long long last_unit = from + done + (cur.left - 1);
                 if (part == 0 && lane == 0) sh_piece[ring][which] = {row_id, ended ? -1 : (int)(last_unit / share / A.rings)};
             }
             started = false;
@@ -741,7 +753,7 @@ __global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedArgs A)
 
 // How a call is cut, from sizes the host knows.
 struct Plan {
-    int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stages, stage_bytes;
+    int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
     int row_mode, grid;
     size_t smem, workspace;
 };
@@ -761,13 +773,12 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     const int keys = unit_keys(p.dm), pitch = ((q8 ? d / 16 : d / 8) + 1) * 16;
     p.stage_bytes = 2 * keys * pitch + (q8 ? 4 * keys * (d / 32) : 0);
     const size_t piece = (size_t)p.warps_per_ring * kRowsPerWarp * (d + 2) * sizeof(float);
-    // as many rings as warps and two stages each allow; a third stage where there is room
+    // as many rings as warps and two stages each allow
     p.rings = max_warps(p.dm) / p.warps_per_ring;
     while (p.rings > 1 && p.rings * 2 * p.stage_bytes > kSmemMost) --p.rings;
-    p.stages = p.rings * 3 * p.stage_bytes <= kSmemMost ? 3 : 2;
-    if (p.rings * p.stages * p.stage_bytes > kSmemMost || (size_t)p.stages * p.stage_bytes < piece)
+    if (p.rings * 2 * p.stage_bytes > kSmemMost || (size_t)2 * p.stage_bytes < piece)
         return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
-    p.smem = (size_t)p.rings * p.stages * p.stage_bytes;
+    p.smem = (size_t)p.rings * 2 * p.stage_bytes;
     const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / keys + 2;
     if (rows > (size_t)INT32_MAX / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
     p.row_mode = units <= (size_t)4 * p.rings;
@@ -865,9 +876,10 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages, a.max_len = (int)max_len, a.heads = (int)heads, a.group = (int)heads / c.kv_heads;
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
     a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp;
-    a.rings = p.rings, a.stages = p.stages, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.min_units = kMinUnits;
+    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.min_units = kMinUnits;
     const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
-    a.page_magic = ((1ull << 32) + per_page - 1) / per_page;  // exact below 2^32 / 256 times 16 keys
+    a.page_magic = per_page == 1 ? 0 : (unsigned)(((1ull << 32) + per_page - 1) / per_page);  // exact below 2^32 / 256 runs of 16 keys
+    a.page_chunks = (unsigned)(c.page_stride / (q8 ? 16 : 8)), a.scale_chunks = (unsigned)(c.scale_stride / 8);
     a.meta = (int*)ws, a.parts = (float*)(ws + (size_t)p.grid * 16);
     cudaError_t e = q8 ? launch_paged<true>(a, p, st) : launch_paged<false>(a, p, st);
     g_trace.launches++;
