@@ -9,12 +9,16 @@
 // Bound: HBM, the cache bytes of the keys in range; everything below serves to keep those copies in flight.
 //
 // Split. Work is counted in units of 32 keys (16 where a row of K is longer than 128 values) of one kv head; a row is one
-// (sequence, kv head). All units of all rows, in order, are cut into equal shares, one per ring: uneven lengths load the
-// GPU evenly and one long sequence uses all of it. A ring is two shared-memory stages of one unit each, filled by
-// cp.async and walked by 1 to 4 warps, each with up to eight of the query heads that share the kv head. A row that lies
-// inside one ring's share is finished there; pieces of rows that cross shares are joined inside the CTA, and pieces that
-// cross CTAs go to the workspace and are joined, in order, by a second kernel. When every row is short, one CTA takes one
-// row and no second kernel runs. The lengths are read on the device: nothing on the host depends on them.
+// (sequence, kv head). All units of all rows, in order, are cut into chunks; a chunk is walked by one ring: two
+// shared-memory stages of one unit each, filled by cp.async and read by 1 to 4 warps, each with up to eight of the query
+// heads that share the kv head. A row that lies inside one chunk is finished there; pieces of rows that cross chunks go to
+// the workspace and a second kernel joins them in order. The chunks are fixed by the lengths, so a result does not depend on
+// which ring walked what. Small calls have one chunk per ring. Large ones give each ring one chunk of three quarters of its
+// fair share and hand out the rest in small ones as rings become free: SMs differ by a fifth in the rate at which memory
+// serves them (64 f16 sequences of up to 8000 tokens: equal shares took 137 to 195 us per SM). A first kernel then adds up
+// the lengths and clears the hand-out counter. When every row is short, one CTA takes one row, its rings' pieces are joined
+// in shared memory, and that kernel is the only one. The lengths are read on the device: nothing on the host depends on
+// them.
 //
 // Copies. The keys of a stage are refilled as soon as the scores are taken, the values after the second product: nearly
 // two units per ring are in flight at any time from two stages' room.
@@ -64,12 +68,15 @@ struct PagedArgs {
     int span;          // query heads of one row
     int warps_per_ring, heads_per_warp, rings;
     int stage_bytes;
-    int row_mode;      // one CTA per row; else shares of at least min_units
-    int min_units;
+    int row_mode;      // one CTA per row
+    int dynamic;       // the plan kernel has run: `sums` holds the units before each sequence, `next` counts handed-out chunks
+    int min_units;     // per chunk
     unsigned page_magic;                  // index of 16 keys / 16-key runs of a page = umulhi(index, page_magic); 0: one run a page
     unsigned page_chunks, scale_chunks;   // 16-byte chunks from page to page
-    int* meta;         // [grid][2]: the row whose beginning CTA c holds in part 1 (-1: none), the last CTA with a piece of it (in part 0)
-    float* parts;      // [grid][2 + rings][warps_per_ring * 8][d + 2]: o, then max and sum; part 2 + r: the first piece of ring r
+    int* next;
+    int* sums;         // [n_seqs + 1]
+    int2* meta;        // per chunk: the row that begins in it and ends in a later one (-1: none), the chunk of the row's end
+    float* parts;      // per chunk [2][warps_per_ring * 8][d + 2] (o, then max and sum): a row that began earlier, a row that ends later
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -155,11 +162,23 @@ struct Cursor {
     }
 };
 
-// Partial results of a row inside the CTA: two per ring, one of a row that began in an earlier share (kept in the
-// workspace; with a CTA per row, on the ring's stages, like the other) and one of a row that began here and ends later.
-struct Piece {
-    int row;   // -1: none
-    int last;  // the CTA that holds the row's last unit; -1: the unit is in this piece
+// How `total` units are cut: `big` units for each of the rings, then chunks of `small`.
+struct Cut {
+    int total, rings, big, small;
+    __device__ __forceinline__ Cut(const PagedArgs& A, int total_, int rings_) : total(total_), rings(rings_) {
+        const int fair = (total + rings - 1) / rings;
+        big = max(A.min_units, A.dynamic ? fair - fair / 4 : fair);
+        small = max(A.min_units, fair / 8);
+    }
+    // the first unit of chunk c, or the end of all
+    __device__ __forceinline__ int begin(int c) const {
+        const long long u = c <= rings ? (long long)c * big : (long long)rings * big + (long long)(c - rings) * small;
+        return (int)(u < total ? u : total);
+    }
+    __device__ __forceinline__ int chunk_of(int unit) const {
+        const long long over = unit - (long long)rings * big;
+        return over < 0 ? unit / big : rings + (int)(over / small);
+    }
 };
 
 // The scales of one key (or value) row: nb = d / 32 halves, in registers as pairs.
@@ -184,10 +203,11 @@ __device__ __forceinline__ void load_scales(const __half* row, int nb, uint32_t 
 template <bool Q8, int DM, bool EXACT>
 __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const __grid_constant__ PagedArgs A) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Piece sh_piece[kMaxRings][2];
+    __shared__ int sh_next[kMaxRings][2];
     pdl_wait_then_release();
     constexpr int UK = unit_keys(DM), NT = UK / 8;  // keys of a unit, and groups of eight of them
     constexpr int KS = DM / 16, NB = DM / 32;       // 16-value steps and 32-value blocks of a row
+    const bool dynamic = !Q8 && A.dynamic;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int ring = warp / A.warps_per_ring, part = warp - ring * A.warps_per_ring;
@@ -201,37 +221,42 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     const int k_scale_at = 2 * UK * pitch, v_scale_at = k_scale_at + UK * 2 * nb;
     uint8_t* ring_base = smem + (size_t)ring * 2 * A.stage_bytes;
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring_base);
-    auto piece_ptr = [&](int rg, int which) {
-        return which == 0 && !A.row_mode ? A.parts + ((size_t)blockIdx.x * (2 + A.rings) + 2 + rg) * piece_floats
-                                         : reinterpret_cast<float*>(smem + (size_t)rg * 2 * A.stage_bytes);
+    auto ring_sync = [&]() {
+        if (A.warps_per_ring == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(ring + 1), "r"(A.warps_per_ring * 32) : "memory");
     };
 
-    // ---- this ring's share
+    // ---- this ring's first chunk
     Cursor<UK> cur;
-    int count, share = 1;
-    long long from = 0;
-    if (A.row_mode) {
-        cur.s = blockIdx.x / rows_per_seq, cur.r = blockIdx.x - cur.s * rows_per_seq;
-        key_range(A, cur.s, cur.first, cur.end);
-        const int units = cur.units(), u = units * ring / A.rings;  // a row of few units
-        count = units * (ring + 1) / A.rings - u;
-        cur.start_row(u);
-    } else {
+    int count, chunk = blockIdx.x * A.rings + ring;
+    auto units_total = [&]() {
+        if (A.row_mode) return 1;
+        if (dynamic) return A.sums[A.n_seqs];
         int mine = 0;
         for (int s = lane; s < A.n_seqs; s += 32) {
             int first, end;
             key_range(A, s, first, end);
             mine += units_of<UK>(first, end);
         }
-        const int total = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine) * rows_per_seq;
-        const int workers = gridDim.x * A.rings;
-        share = max(A.min_units, (int)(((long long)total + workers - 1) / workers));
-        from = (long long)(blockIdx.x * A.rings + ring) * share;
-        count = (int)max(0ll, min((long long)share, total - from));
-        cur = {0, 0, 1, 0, 0, 0};
-        if (count > 0) {
-            // the sequence that holds unit `from`
-            int before = 0;
+        return (int)__reduce_add_sync(0xffffffffu, (unsigned)mine) * rows_per_seq;
+    };
+    const Cut split(A, units_total(), gridDim.x * A.rings);
+    // unit `from` of all
+    auto locate = [&](Cursor<UK>& c, int from) {
+        if (dynamic) {
+            // the last sequence with sums[s] <= from: 32 places at a time
+            int lo = 0, hi = A.n_seqs;  // sums[lo] <= from < sums[hi]
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 31) / 32, at = min(lo + lane * step, hi);
+                const unsigned below = __ballot_sync(0xffffffffu, at < hi && A.sums[at] <= from);
+                const int l = 31 - __clz(below);
+                hi = min(lo + (l + 1) * step, hi);
+                lo += l * step;
+            }
+            c.s = lo;
+            key_range(A, lo, c.first, c.end);
+            from -= A.sums[lo];
+        } else {
             for (int s0 = 0; s0 < A.n_seqs; s0 += 32) {
                 int first = 0, end = 0, n = 0;
                 if (s0 + lane < A.n_seqs) key_range(A, s0 + lane, first, end), n = units_of<UK>(first, end) * rows_per_seq;
@@ -241,27 +266,56 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                     const int up = __shfl_up_sync(0xffffffffu, sum, o);
                     if (lane >= o) sum += up;
                 }
-                const unsigned over = __ballot_sync(0xffffffffu, (long long)before + sum > from);
+                const unsigned over = __ballot_sync(0xffffffffu, sum > from);
                 if (over) {
                     const int l = __ffs(over) - 1;
-                    const int local = (int)(from - before) - __shfl_sync(0xffffffffu, sum - n, l);
-                    cur.s = s0 + l;
-                    cur.first = __shfl_sync(0xffffffffu, first, l), cur.end = __shfl_sync(0xffffffffu, end, l);
-                    cur.r = local / cur.units();
-                    cur.start_row(local - cur.r * cur.units());
+                    from -= __shfl_sync(0xffffffffu, sum - n, l);
+                    c.s = s0 + l;
+                    c.first = __shfl_sync(0xffffffffu, first, l), c.end = __shfl_sync(0xffffffffu, end, l);
                     break;
                 }
-                before += __shfl_sync(0xffffffffu, sum, 31);
+                from -= __shfl_sync(0xffffffffu, sum, 31);
             }
         }
+        const int units = c.units();
+        c.r = from / units;
+        c.start_row(from - c.r * units);
+    };
+    cur = {0, 0, 1, 0, 0, 0};
+    if (A.row_mode) {
+        cur.s = blockIdx.x / rows_per_seq, cur.r = blockIdx.x - cur.s * rows_per_seq;
+        key_range(A, cur.s, cur.first, cur.end);
+        const int units = cur.units(), u = units * ring / A.rings;  // a row of few units
+        count = units * (ring + 1) / A.rings - u;
+        cur.start_row(u);
+    } else {
+        const int from = split.begin(chunk);
+        count = split.begin(chunk + 1) - from;
+        if (count > 0) locate(cur, from);
+        else if (part == 0 && lane == 0 && !dynamic) A.meta[chunk] = make_int2(-1, -1);
     }
-    if (part == 0 && lane < 2) sh_piece[ring][lane] = {-1, -1};
+    // The chunk after this one is asked for long before it is needed, and the answer is posted to the ring's warps a unit
+    // later, when it has arrived; two places, so that none of them finds its answer overwritten. Behind the last chunk of all
+    // nobody asks: it may be shorter than the three units that keep asking, posting and reading a barrier apart.
+    int asked = 0, answer = 0;
+    bool more = false, to_post = false;
+    auto ask = [&](int end) {
+        more = end < split.total;
+        if (!more) return;
+        if (part == 0 && lane == 0) answer = split.rings + atomicAdd(A.next, 1);
+        ++asked;
+        to_post = true;
+    };
+    if (dynamic && count > 0) ask(split.begin(chunk) + count);
 
     // ---- copies. `ahead` is the unit copied next; its pages are looked up a step before they are needed. A unit is one or two
     // runs of 16 keys, each inside one page: run x starts `run[x]` chunks into k and v (its scales `srun[x]` chunks into theirs).
     constexpr int RUNS = UK / kSub;
     Cursor<UK> ahead = cur;
     int left = count;
+    // the chunk that `ahead` has entered and the ring is yet to begin (a chunk is longer than the two units between them)
+    Cursor<UK> coming = cur;
+    int coming_chunk = -1, coming_count = 0;
     unsigned have = 0;  // runs of the unit to copy that exist
     unsigned gone_new = 0, gone_next = 0, gone_now = 0;  // runs whose page is no page: of the unit to copy, and of the two in the stages
     int pg[RUNS], pu[RUNS];
@@ -334,14 +388,26 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     };
     auto step_ahead = [&]() {
         gone_now = gone_next, gone_next = gone_new;
+        if (to_post) {
+            if (part == 0 && lane == 0) sh_next[ring][(asked - 1) & 1] = answer;
+            to_post = false;
+        }
         if (--left > 0) {
             if (ahead.next(A, rows_per_seq)) enter_row();
             look_up();
+        } else if (left == 0 && more) {
+            const int c = sh_next[ring][(asked - 1) & 1];
+            const int from = split.begin(c), n = split.begin(c + 1) - from;
+            more = false;
+            if (n > 0) {
+                locate(ahead, from);
+                ask(from + n);
+                left = n;
+                coming = ahead, coming_chunk = c, coming_count = n;
+                enter_row();
+                look_up();
+            }
         }
-    };
-    auto ring_sync = [&]() {
-        if (A.warps_per_ring == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(ring + 1), "r"(A.warps_per_ring * 32) : "memory");
     };
     if (count > 0) enter_row(), look_up();
 #pragma unroll
@@ -363,7 +429,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     const uint32_t k_lane = (uint32_t)(((mi >> 1) * 8 + mr) * pitch + (mi & 1) * 16);
     const uint32_t v_lane = (uint32_t)(((mi & 1) * 8 + mr) * pitch + (mi >> 1) * 16);
 
-    for (int done = 0; done < count; ++done) {
+    int done = 0;
+    while (count > 0) {
         if (!started) {
             started = true;
             begun_here = cur.key == cur.first / UK * UK;
@@ -598,19 +665,17 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         step_ahead();
         stage_at = A.stage_bytes - stage_at;
 
-        const bool ended = cur.left == 1;
-        if (ended || done + 1 == count) {
+        const bool ended = cur.left == 1, chunk_over = ++done == count;
+        if (ended || chunk_over) {
             l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
             l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-            const int row_id = cur.s * rows_per_seq + cur.r;
             const int in_row = part * A.heads_per_warp + g, kvh = cur.r / A.passes, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
             const bool finished = begun_here && ended;
             const bool live = g < A.heads_per_warp && in_row < A.span && in_group < A.group;
             const int which = begun_here ? 1 : 0;
             const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
-            // a piece on the stages is the share's last: all warps are done with them
-            if (!finished && (which == 1 || A.row_mode)) ring_sync();
-            float* pc = piece_ptr(ring, which);
+            if (A.row_mode && !finished) ring_sync();  // the piece lands on the ring's stages: all its warps are done with them
+            float* pc = A.row_mode ? reinterpret_cast<float*>(ring_base) : A.parts + ((size_t)chunk * 2 + which) * piece_floats;
             float* dst = finished ? A.out + at * d : pc + (size_t)(part * kRowsPerWarp + g) * d;
             const float f = finished ? (l_run > 0.0f || l_run != l_run ? v_unit / l_run : 0.0f) : v_unit;
             if (live || !finished) {
@@ -633,133 +698,240 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             } else {
                 float* ml = pc + (size_t)prow * d + (part * kRowsPerWarp + g) * 2;
                 if (t == 0) ml[0] = m_run, ml[1] = l_run;
-                const long long last_unit = from + done + (cur.left - 1);
-                if (part == 0 && lane == 0) sh_piece[ring][which] = {row_id, ended ? -1 : (int)(last_unit / share / A.rings)};
+                if (which == 1 && !A.row_mode && part == 0 && lane == 0)
+                    A.meta[chunk] = make_int2(cur.s * rows_per_seq + cur.r, split.chunk_of(split.begin(chunk) + done - 1 + cur.left - 1));
             }
+            if (chunk_over && !A.row_mode && (finished || which == 0) && part == 0 && lane == 0) A.meta[chunk] = make_int2(-1, -1);
             started = false;
         }
-        cur.next(A, rows_per_seq);
-    }
-
-    // ---- join the pieces inside the CTA, in order (a warp per head row, a lane per piece for the weights, then four values a
-    // lane); what still lacks its beginning or its end goes to the workspace
-    __syncthreads();
-    const int entries = 2 * A.rings, warps = blockDim.x >> 5;
-    Piece mine{-1, -1};
-    if (lane < entries) mine = sh_piece[lane >> 1][lane & 1];
-    int tail_row = -1, tail_last = 0;
-    for (unsigned todo = __ballot_sync(0xffffffffu, mine.row >= 0); todo;) {
-        const int e0 = __ffs(todo) - 1;
-        const int row = __shfl_sync(0xffffffffu, mine.row, e0);
-        const unsigned run = __ballot_sync(0xffffffffu, mine.row == row);
-        const int e1 = 31 - __clz(run);
-        const bool begun = (e0 & 1) != 0, ended = __shfl_sync(0xffffffffu, mine.last, e1) < 0;
-        if (begun && !ended) tail_row = row, tail_last = __shfl_sync(0xffffffffu, mine.last, e0);
-        const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
-        for (int pr = warp; pr < prow; pr += warps) {
-            float m = -INFINITY, l = 0.0f;
-            const bool in = (run >> lane) & 1;
-            if (in) {
-                const float* ml = piece_ptr(lane >> 1, lane & 1) + (size_t)prow * d + pr * 2;
-                m = ml[0], l = ml[1];
-            }
-            float m_all = m;
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
-            const float f = m == -INFINITY ? 0.0f : ex2((m - m_all) * kLog2e);
-            l *= f;
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-            const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
-            const bool live = (pr & 7) < A.heads_per_warp && in_row < A.span && in_group < A.group;
-            const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
-            const bool finished = begun && ended;
-            float* part_out = A.parts + ((size_t)blockIdx.x * (2 + A.rings) + (begun ? 1 : 0)) * piece_floats;
-            float* dst = finished ? A.out + at * d : part_out + (size_t)pr * d;
-            const float inv = !finished ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            for (int i0 = 0; i0 < d; i0 += 128) {
-                const int i = i0 + lane * 4;
-                float4 a = make_float4(0, 0, 0, 0);
-                for (unsigned rest = run; rest; rest &= rest - 1) {
-                    const int e = __ffs(rest) - 1;
-                    const float fe = __shfl_sync(0xffffffffu, f, e);
-                    if (i < d) {
-                        const float4 x = *reinterpret_cast<const float4*>(piece_ptr(e >> 1, e & 1) + (size_t)pr * d + i);
-                        a.x = fmaf(x.x, fe, a.x), a.y = fmaf(x.y, fe, a.y), a.z = fmaf(x.z, fe, a.z), a.w = fmaf(x.w, fe, a.w);
-                    }
-                }
-                if (i < d && (live || !finished)) *reinterpret_cast<float4*>(dst + i) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            }
-            if (lane == 0) {
-                if (!finished) part_out[(size_t)prow * d + pr * 2] = m_all, part_out[(size_t)prow * d + pr * 2 + 1] = l;
-                else if (A.stats && live) A.stats[at * 2] = l > 0.0f ? m_all : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
-            }
+        if (!chunk_over) {
+            cur.next(A, rows_per_seq);
+        } else {
+            done = 0, count = 0;
+            if (coming_chunk >= 0) cur = coming, chunk = coming_chunk, count = coming_count, coming_chunk = -1;
         }
-        todo &= ~run;
     }
-    if (!A.row_mode && threadIdx.x == 0) A.meta[blockIdx.x * 2] = tail_row, A.meta[blockIdx.x * 2 + 1] = tail_last;
+    if (!A.row_mode) return;
+
+    // ---- join the rings' pieces of this CTA's row, in order: a warp per head row, a lane per piece for the weights, then four
+    // values a lane. A row of one unit was finished by its ring.
+    __syncthreads();
+    const int s = blockIdx.x / rows_per_seq, r = blockIdx.x - s * rows_per_seq, kvh = r / A.passes;
+    int first, end;
+    key_range(A, s, first, end);
+    const int units = units_of<UK>(first, end), warps = blockDim.x >> 5;
+    if (units == 1 || A.rings == 1) return;
+    const size_t ring_floats = (size_t)2 * A.stage_bytes / sizeof(float);
+    const float* pieces = reinterpret_cast<const float*>(smem);
+    const bool in = lane < A.rings && units * (lane + 1) / A.rings > units * lane / A.rings;
+    for (int pr = warp; pr < prow; pr += warps) {
+        const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
+        if ((pr & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) continue;
+        float m = -INFINITY, l = 0.0f;
+        if (in) m = pieces[lane * ring_floats + prow * d + pr * 2], l = pieces[lane * ring_floats + prow * d + pr * 2 + 1];
+        float m_all = m;
+#pragma unroll
+        for (int x = kMaxRings / 2; x > 0; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
+        m_all = __shfl_sync(0xffffffffu, m_all, 0);
+        const float f = m == -INFINITY ? 0.0f : ex2((m - m_all) * kLog2e);
+        l = in ? l * f : 0.0f;
+#pragma unroll
+        for (int x = kMaxRings / 2; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        l = __shfl_sync(0xffffffffu, l, 0);
+        const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const unsigned present = __ballot_sync(0xffffffffu, in);
+#pragma unroll
+        for (int i0 = 0; i0 < DM; i0 += 128) {
+            const int i = i0 + lane * 4;
+            float4 a = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+            for (int e = 0; e < A.rings; ++e) {
+                const float fe = __shfl_sync(0xffffffffu, f, e);
+                if (i < d && ((present >> e) & 1)) {
+                    const float4 x = *reinterpret_cast<const float4*>(pieces + e * ring_floats + (size_t)pr * d + i);
+                    a.x = fmaf(x.x, fe, a.x), a.y = fmaf(x.y, fe, a.y), a.z = fmaf(x.z, fe, a.z), a.w = fmaf(x.w, fe, a.w);
+                }
+            }
+            if (i < d) *reinterpret_cast<float4*>(A.out + at * d + i) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+        }
+        if (lane == 0 && A.stats) A.stats[at * 2] = l > 0.0f ? m_all : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
+    }
 }
 
-// Rows that cross CTAs: block (c, head row) joins the row whose beginning CTA c holds with the pieces of the CTAs after it.
-// The pieces are added in order by four warps (every fourth piece each), the warps' sums in warp order.
-__global__ void __launch_bounds__(128) attn_paged_join_kernel(const PagedArgs A) {
-    __shared__ __align__(16) float sh_o[4][kKvMaxD];
-    __shared__ float sh_m[4], sh_l[4];
+// The units before each sequence, and a fresh hand-out counter: one CTA, 1024 sequences at a time.
+template <int UK>
+__global__ void __launch_bounds__(1024) attn_paged_plan_kernel(const PagedArgs A) {
+    __shared__ int sh_warp[32];
     pdl_wait_then_release();
-    const int c0 = blockIdx.x, pr = blockIdx.y, d = A.c.d;
-    const int row = A.meta[c0 * 2];
-    if (row < 0) return;
-    const int rows_per_seq = A.c.kv_heads * A.passes;
-    const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
-    const int wp = pr >> 3, in_row = wp * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
-    if ((pr & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) return;
-    const int prow = A.warps_per_ring * kRowsPerWarp, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const size_t piece_floats = (size_t)prow * (d + 2);
-    const int n = A.meta[c0 * 2 + 1] - c0 + 1;
-    auto piece = [&](int i) { return A.parts + ((size_t)(c0 + i) * (2 + A.rings) + (i == 0 ? 1 : 0)) * piece_floats; };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 128) m = fmaxf(m, piece(i)[(size_t)prow * d + pr * 2]);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows_per_seq = A.c.kv_heads * A.passes;
+    if (threadIdx.x == 0) *A.next = 0;
+    int before = 0;
+    for (int s0 = 0; s0 < A.n_seqs; s0 += 1024) {
+        const int s = s0 + threadIdx.x;
+        int first, end, n = 0;
+        if (s < A.n_seqs) key_range(A, s, first, end), n = units_of<UK>(first, end) * rows_per_seq;
+        int sum = n;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    if (lane == 0) sh_m[w] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-    float l = 0.0f;
-    for (int d0 = 0; d0 < d; d0 += 128) {
-        const int dim = d0 + lane * 4;
-        float4 a = make_float4(0, 0, 0, 0);
-        for (int i = w; i < n; i += 4) {
-            const float* pc = piece(i);
-            const float pm = pc[(size_t)prow * d + pr * 2];
-            const float f = pm == -INFINITY ? 0.0f : ex2((pm - m) * kLog2e);
-            if (d0 == 0) l += pc[(size_t)prow * d + pr * 2 + 1] * f;
-            if (dim < d) {
-                const float4 x = *reinterpret_cast<const float4*>(pc + (size_t)pr * d + dim);
-                a.x = fmaf(x.x, f, a.x), a.y = fmaf(x.y, f, a.y), a.z = fmaf(x.z, f, a.z), a.w = fmaf(x.w, f, a.w);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 31) sh_warp[warp] = sum;
+        __syncthreads();
+        int base = lane < warp ? sh_warp[lane] : 0, all = sh_warp[lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o), all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (s < A.n_seqs) A.sums[s] = before + base + sum - n;
+        before += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) A.sums[A.n_seqs] = before;
+}
+
+// Rows that cross chunks. Work items are (chunk, head row); a block of eight warps first finds, 256 at a time, which of its
+// items begin a row that ends in a later chunk. A row of up to 16 pieces is joined by one warp, a longer one by all eight,
+// every eighth piece a warp, and the warps' results in warp order. Loads are what bounds this: a lane loads the maximum and
+// the sum of one piece, 32 pieces at once, and then four values of eight pieces before any of them is used.
+constexpr int kJoinWarps = 8, kJoinAlone = 16;
+struct Joined {
+    float m, l;
+    float4 a[kKvMaxD / 128];
+    __device__ __forceinline__ void scale(float f) {
+        l *= f;
+#pragma unroll
+        for (int x = 0; x < kKvMaxD / 128; ++x) a[x].x *= f, a[x].y *= f, a[x].z *= f, a[x].w *= f;
+    }
+};
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const PagedArgs A, int rings) {
+    __shared__ __align__(16) float sh_o[kJoinWarps][kKvMaxD];
+    __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps];
+    __shared__ int4 sh_todo[kJoinWarps * 32];
+    __shared__ int sh_count[2];
+    pdl_wait_then_release();
+    const int d = A.c.d, w = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = kJoinWarps * 32;
+    const int prow = A.warps_per_ring * kRowsPerWarp, rows_per_seq = A.c.kv_heads * A.passes;
+    const size_t piece_floats = (size_t)prow * (d + 2);
+    int chunks = rings;
+    if (A.dynamic) {
+        const Cut split(A, A.sums[A.n_seqs], rings);
+        chunks = split.chunk_of(split.total - 1) + 1;
+    }
+    // pieces from, from + step, .. of item (chunk, head row, row, last chunk)
+    auto join = [&](const int4& it, int from, int step) {
+        const int n = it.w - it.x + 1, pr = it.y;
+        Joined j{-INFINITY, 0.0f, {}};
+        for (int i0 = from; i0 < n; i0 += 32 * step) {
+            const int mine = i0 + lane * step, count = min(32, (n - i0 + step - 1) / step);
+            auto piece = [&](int i) { return A.parts + ((size_t)(it.x + i) * 2 + (i == 0 ? 1 : 0)) * piece_floats; };
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (mine < n) ml = *reinterpret_cast<const float2*>(piece(mine) + (size_t)prow * d + pr * 2);
+            float m = fmaxf(j.m, ml.x);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            j.scale(j.m == -INFINITY ? 0.0f : ex2((j.m - m) * kLog2e));
+            j.m = m;
+            const float f = ml.x == -INFINITY ? 0.0f : ex2((ml.x - m) * kLog2e);
+            float l = ml.y * f;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            j.l += l;
+            for (int k0 = 0; k0 < count; k0 += 8) {
+#pragma unroll
+                for (int x = 0; x < kKvMaxD / 128; ++x) {
+                    const int dim = x * 128 + lane * 4;
+                    if (x * 128 >= d) break;
+                    float4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        v[k] = k0 + k < count && dim < d ? *reinterpret_cast<const float4*>(piece(i0 + (k0 + k) * step) + (size_t)pr * d + dim) : make_float4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float fk = __shfl_sync(0xffffffffu, f, k0 + k);
+                        if (k0 + k < count) j.a[x].x = fmaf(v[k].x, fk, j.a[x].x), j.a[x].y = fmaf(v[k].y, fk, j.a[x].y), j.a[x].z = fmaf(v[k].z, fk, j.a[x].z), j.a[x].w = fmaf(v[k].w, fk, j.a[x].w);
+                    }
+                }
             }
         }
-        if (dim < d) *reinterpret_cast<float4*>(&sh_o[w][dim]) = a;
+        return j;
+    };
+    // where item `it` goes: the head's place in out, or -1
+    auto place_of = [&](const int4& it) {
+        const int s = it.z / rows_per_seq, r = it.z - s * rows_per_seq, kvh = r / A.passes;
+        const int in_row = (it.y >> 3) * A.heads_per_warp + (it.y & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
+        if ((it.y & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) return -1ll;
+        return (long long)s * A.heads + (long long)kvh * A.group + in_group;
+    };
+    const long long items = (long long)chunks * prow;
+    for (long long base = blockIdx.x; base < items; base += (long long)gridDim.x * threads) {
+        if (threadIdx.x < 2) sh_count[threadIdx.x] = 0;
+        __syncthreads();
+        const long long item = base + (long long)threadIdx.x * gridDim.x;
+        if (item < items) {
+            const int c = (int)(item / prow);
+            const int2 m = A.meta[c];
+            // from the front those for one warp, from the back those for all: any order, the items are independent
+            if (m.x >= 0) {
+                const int4 it = make_int4(c, (int)(item - (long long)c * prow), m.x, m.y);
+                if (m.y - c + 1 <= kJoinAlone) sh_todo[atomicAdd(&sh_count[0], 1)] = it;
+                else sh_todo[threads - 1 - atomicAdd(&sh_count[1], 1)] = it;
+            }
+        }
+        __syncthreads();
+        const int alone = sh_count[0], together = sh_count[1];
+        for (int k = w; k < alone; k += kJoinWarps) {
+            const int4 it = sh_todo[k];
+            const long long at = place_of(it);
+            if (at < 0) continue;
+            const Joined j = join(it, 0, 1);
+            const float inv = j.l > 0.0f || j.l != j.l ? 1.0f / j.l : 0.0f;
+#pragma unroll
+            for (int x = 0; x < kKvMaxD / 128; ++x) {
+                const int dim = x * 128 + lane * 4;
+                if (dim < d) *reinterpret_cast<float4*>(A.out + at * d + dim) = make_float4(j.a[x].x * inv, j.a[x].y * inv, j.a[x].z * inv, j.a[x].w * inv);
+            }
+            if (A.stats && lane == 0) A.stats[at * 2] = j.l > 0.0f ? j.m : kNegBig, A.stats[at * 2 + 1] = j.l * (1.0f / 32768.0f);
+        }
+        for (int k = 0; k < together; ++k) {
+            const int4 it = sh_todo[threads - 1 - k];
+            const long long at = place_of(it);
+            if (at < 0) continue;
+            const Joined j = join(it, w, kJoinWarps);
+#pragma unroll
+            for (int x = 0; x < kKvMaxD / 128; ++x)
+                if (x * 128 + lane * 4 < d) *reinterpret_cast<float4*>(&sh_o[w][x * 128 + lane * 4]) = j.a[x];
+            if (lane == 0) sh_m[w] = j.m, sh_l[w] = j.l;
+            __syncthreads();
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, sh_m[i]);
+            float f[kJoinWarps];
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) f[i] = sh_m[i] == -INFINITY ? 0.0f : ex2((sh_m[i] - m) * kLog2e), l += sh_l[i] * f[i];
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            for (int i = threadIdx.x; i < d; i += threads) {
+                float a = 0.0f;
+#pragma unroll
+                for (int x = 0; x < kJoinWarps; ++x) a += sh_o[x][i] * f[x];
+                A.out[at * d + i] = a * inv;
+            }
+            if (A.stats && threadIdx.x == 0) A.stats[at * 2] = l > 0.0f ? m : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
+            __syncthreads();  // sh_o, sh_m and sh_l are free for the next item
+        }
+        __syncthreads();
     }
-    if (lane == 0) sh_l[w] = l;
-    __syncthreads();
-    l = ((sh_l[0] + sh_l[1]) + sh_l[2]) + sh_l[3];
-    const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
-    for (int i = threadIdx.x; i < d; i += 128) {
-        const float a = ((sh_o[0][i] + sh_o[1][i]) + sh_o[2][i]) + sh_o[3][i];
-        A.out[at * d + i] = l > 0.0f || l != l ? a / l : 0.0f;
-    }
-    if (A.stats && threadIdx.x == 0) A.stats[at * 2] = l > 0.0f ? m : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
 }
 
 // How a call is cut, from sizes the host knows.
 struct Plan {
     int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
-    int row_mode, grid;
-    size_t smem, workspace;
+    int row_mode, dynamic, grid, chunks;
+    size_t smem, sums_at, meta_at, parts_at, workspace;
 };
 
-// At least two units of a row per share: below that the joins cost more than the copies they spread.
-constexpr int kMinUnits = 2;
+// A chunk has at least two units (a ring's depth of copies; below that the joins cost more than the copies they spread),
+// three where chunks are handed out.
+constexpr int kMinUnits = 2, kMinUnitsDynamic = 3;
 
 int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max_len, int sm_count, Plan* out) {
     Plan p;
@@ -782,9 +954,18 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / keys + 2;
     if (rows > (size_t)INT32_MAX / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
     p.row_mode = units <= (size_t)4 * p.rings;
-    const size_t shares = (rows * units + kMinUnits - 1) / kMinUnits, ctas = (shares + p.rings - 1) / p.rings;
+    const size_t most = rows * units, rings_all = (size_t)sm_count * p.rings;
+    p.dynamic = !p.row_mode && !q8 && most >= 48 * rings_all;
+    const size_t shares = (most + kMinUnits - 1) / kMinUnits, ctas = (shares + p.rings - 1) / p.rings;
     p.grid = p.row_mode ? (int)rows : (int)(ctas < (size_t)sm_count ? ctas : (size_t)sm_count);
-    p.workspace = p.row_mode ? 0 : (size_t)p.grid * (16 + (2 + p.rings) * piece);
+    // one chunk per ring; handed out, the rest (a quarter of the fair shares) in chunks of an eighth of one or of three units:
+    // (fair / 4) / (fair / 8) rounded down is at most 5 / 1, and 3 where the least size binds
+    p.chunks = p.grid * p.rings * (p.dynamic ? 6 : 1);
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    p.sums_at = 256;
+    p.meta_at = p.sums_at + (p.dynamic ? up((n_seqs + 1) * sizeof(int)) : 0);
+    p.parts_at = p.meta_at + up(p.chunks * sizeof(int2));
+    p.workspace = p.row_mode ? 0 : p.parts_at + (size_t)p.chunks * 2 * piece;
     *out = p;
     return FQ_OK;
 }
@@ -876,15 +1057,22 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages, a.max_len = (int)max_len, a.heads = (int)heads, a.group = (int)heads / c.kv_heads;
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
     a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp;
-    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.min_units = kMinUnits;
+    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.dynamic = p.dynamic;
+    a.min_units = p.dynamic ? kMinUnitsDynamic : kMinUnits;
     const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
     a.page_magic = per_page == 1 ? 0 : (unsigned)(((1ull << 32) + per_page - 1) / per_page);  // exact below 2^32 / 256 runs of 16 keys
     a.page_chunks = (unsigned)(c.page_stride / (q8 ? 16 : 8)), a.scale_chunks = (unsigned)(c.scale_stride / 8);
-    a.meta = (int*)ws, a.parts = (float*)(ws + (size_t)p.grid * 16);
-    cudaError_t e = q8 ? launch_paged<true>(a, p, st) : launch_paged<false>(a, p, st);
+    a.next = (int*)ws, a.sums = (int*)(ws + p.sums_at), a.meta = (int2*)(ws + p.meta_at), a.parts = (float*)(ws + p.parts_at);
+    cudaError_t e = cudaSuccess;
+    if (p.dynamic) {
+        e = launch_pdl(unit_keys(p.dm) == 32 ? attn_paged_plan_kernel<32> : attn_paged_plan_kernel<16>, dim3(1), dim3(1024), 0, st, a);
+        g_trace.launches++;
+    }
+    if (e == cudaSuccess) e = q8 ? launch_paged<true>(a, p, st) : launch_paged<false>(a, p, st);
     g_trace.launches++;
     if (e == cudaSuccess && !p.row_mode) {
-        e = launch_pdl(attn_paged_join_kernel, dim3((unsigned)p.grid, (unsigned)(p.warps_per_ring * kRowsPerWarp)), dim3(128), 0, st, a);
+        const size_t items = (size_t)p.chunks * p.warps_per_ring * kRowsPerWarp, blocks = (size_t)ctx->sm_count * 4;
+        e = launch_pdl(attn_paged_join_kernel, dim3((unsigned)(items < blocks ? items : blocks)), dim3(kJoinWarps * 32), 0, st, a, p.grid * p.rings);
         g_trace.launches++;
     }
     if (own) dev_free_on(own, st);

@@ -165,6 +165,33 @@ def test_shared_prefix_pages(P):
     check_attention(cache, mixed, q, got, 0.125)
 
 
+@pytest.mark.parametrize("kind,heads,kv,d", [("q8_0", 2, 1, 128), ("f16", 16, 1, 128), ("q8_0", 20, 1, 64), ("f16", 32, 1, 64), ("f16", 12, 1, 256)])
+@pytest.mark.parametrize("rings", [2, 4, 6, 8, 11, 12])
+@pytest.mark.parametrize("over", [1, 2, 3, 5])
+def test_last_chunks_of_every_size(P, kind, heads, kv, d, rings, over):
+    """Very short sequences under a table for long ones: work is handed out in chunks of three units (a unit per sequence),
+    and the last chunk has one, two or three, for whatever number of rings an SM holds."""
+    import torch
+
+    rng = np.random.default_rng(24)
+    n = P.sm_count() * rings * 3 + over
+    lens = [int(x) for x in rng.integers(0, 4, n)]
+    cache = Cache(P, kind, lens, 16, kv, d, rng)
+    rows = cache.fill(rng)
+    wide = torch.full((n, 128), -1, dtype=torch.int32).cuda()
+    wide[:, :1] = cache.table
+    cache.table, cache.max_pages = wide, 128
+    q = rng.standard_normal((n, heads, d)).astype(np.float32)
+    got, _ = cache.attend(q, heads, 0.125)
+    for s in range(n):
+        if lens[s] == 0:
+            assert not got[s].any()
+    some = [0, 1, 2, n - 1, n - 2, n - 3] + [int(x) for x in rng.integers(0, n, 60)]
+    sub = Cache.__new__(Cache)
+    sub.kind, sub.d = kind, d
+    check_attention(sub, [rows[s] for s in some], q[some], got[some], 0.125)
+
+
 @pytest.mark.parametrize("kind", ["f16", "q8_0"])
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 31, 32, 33, 100])
 def test_pages_behind_the_window_may_be_gone(P, kind, window):
