@@ -6,8 +6,7 @@
 // block equals the library's other encoders bit for bit.
 //
 // Bound: HBM. A written value costs 4 bytes read and 2 (f16) or 1.06 (Q8_0) written, a value read back the cache bytes
-// plus 2 or 4. A thread moves eight values (a quarter of a Q8_0 block: its scale is agreed over four lanes), so one
-// instruction reads 32 bytes and writes 16 or 8 with whole sectors per warp.
+// plus 2 or 4. A thread moves eight keys and eight values (a quarter of a Q8_0 block: its scale is agreed over four lanes).
 #include <cuda_fp16.h>
 
 #include "actquant.cuh"
@@ -53,37 +52,39 @@ struct KvRowsArgs {
     const int* pos;
     const int* table;
     int n_seqs, max_pages;
-    int chunks;        // eight-value pieces of a row: kv_heads * d / 8
-    long long total;   // n_tokens * chunks
+    unsigned total;                      // rows * pieces
+    FastDiv pieces, head, page_tokens;   // eight-value pieces of a row (kv_heads * d / 8) and of a head (d / 8)
     int* status;
 };
 
-// Where piece `col` (eight values) of the row lies: an element offset into k or v, and the block's offset into the scales.
-__device__ __forceinline__ void piece_offsets(const KvView& c, const KvSlot& at, int col, size_t& elem, size_t& scale) {
-    const int e = col * 8, head = e / c.d, dim = e - head * c.d;
-    const size_t row = (size_t)head * c.page_tokens + at.slot;
-    elem = (size_t)at.page * c.page_stride + row * c.d + dim;
-    scale = (size_t)at.page * c.scale_stride + row * (c.d >> 5) + (dim >> 5);
+// Where piece `col` (eight values) of the row lies: an element offset into k and v, and the block's offset into the scales.
+__device__ __forceinline__ void piece_offsets(const KvRowsArgs& A, const KvSlot& at, unsigned col, size_t& elem, size_t& scale) {
+    const unsigned head = A.head.div(col), dim = (col - head * A.head.d) * 8;
+    const unsigned row = head * A.c.page_tokens + at.slot;
+    elem = (size_t)at.page * A.c.page_stride + (size_t)row * A.c.d + dim;
+    scale = (size_t)at.page * A.c.scale_stride + row * (A.c.d >> 5) + (dim >> 5);
 }
 
-// blockIdx.y: 0 keys, 1 values
+// A thread writes one piece of the keys and the same piece of the values: their loads do not wait for the page table, and
+// the address arithmetic is done once for both. (A batch of 11 000 tokens of eight heads of 128, written and read back:
+// one piece of one side a thread and plain divisions took 70 us.)
 template <bool Q8>
-__global__ void __launch_bounds__(256) kv_append_kernel(const KvRowsArgs A) {
+__global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ KvRowsArgs A) {
     pdl_wait_then_release();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool side = blockIdx.y != 0;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
     bool live = i < A.total;
-    const int row = live ? (int)(i / A.chunks) : 0, col = live ? (int)(i - (long long)row * A.chunks) : 0;
-    float v[8];
+    const unsigned row = live ? A.pieces.div(i) : 0, col = live ? i - row * A.pieces.d : 0;
+    float k[8], v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.0f;
     KvSlot at{-1, 0};
     if (live) {
-        load8((side ? A.v_in : A.k_in) + (size_t)row * A.row_stride + (size_t)col * 8, v);
-        const int seq = A.seq[row];
+        const int seq = A.seq[row], pos = A.pos[row];
+        load8(A.k_in + (size_t)row * A.row_stride + (size_t)col * 8, k);
+        load8(A.v_in + (size_t)row * A.row_stride + (size_t)col * 8, v);
         live = seq >= 0;
         if (live) {
-            at = kv_slot(A.table, A.n_seqs, A.max_pages, A.c.page_tokens, A.c.n_pages, seq, A.pos[row]);
+            at = kv_slot(A.table, A.n_seqs, A.max_pages, A.page_tokens, A.c.n_pages, seq, pos);
             if (at.page < 0) {
                 *(volatile int*)A.status = FQ_ERR_PAGE;
                 live = false;
@@ -91,60 +92,46 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvRowsArgs A) {
         }
     }
     size_t elem = 0, sc = 0;
-    if (live) piece_offsets(A.c, at, col, elem, sc);
-    uint8_t* out = side ? A.c.v : A.c.k;
+    if (live) piece_offsets(A, at, col, elem, sc);
     if (Q8) {
         // four neighbouring lanes hold a block (a row is whole blocks and the first lane of a warp starts one); every
         // lane takes part in the shuffles, lanes with nothing to write only skip their stores
         int q[8];
-        const uint16_t dh = q8_0_quarter(v, q);
+        uint2 packed;
+        uint16_t dh = q8_0_quarter(k, q);
+        packed.x = pack4(q), packed.y = pack4(q + 4);
         if (live) {
-            uint2 packed;
-            packed.x = pack4(q);
-            packed.y = pack4(q + 4);
-            *reinterpret_cast<uint2*>(out + elem) = packed;
-            if ((threadIdx.x & 3) == 0) reinterpret_cast<uint16_t*>(side ? A.c.v_scale : A.c.k_scale)[sc] = dh;
+            *reinterpret_cast<uint2*>(A.c.k + elem) = packed;
+            if ((threadIdx.x & 3) == 0) reinterpret_cast<uint16_t*>(A.c.k_scale)[sc] = dh;
+        }
+        dh = q8_0_quarter(v, q);
+        packed.x = pack4(q), packed.y = pack4(q + 4);
+        if (live) {
+            *reinterpret_cast<uint2*>(A.c.v + elem) = packed;
+            if ((threadIdx.x & 3) == 0) reinterpret_cast<uint16_t*>(A.c.v_scale)[sc] = dh;
         }
     } else if (live) {
-        __half2 h[4];
+        __half2 h[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        *reinterpret_cast<uint4*>(out + elem * 2) = *reinterpret_cast<const uint4*>(h);
+        for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(k[2 * j], k[2 * j + 1]), h[4 + j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        *reinterpret_cast<uint4*>(A.c.k + elem * 2) = *reinterpret_cast<const uint4*>(h);
+        *reinterpret_cast<uint4*>(A.c.v + elem * 2) = *reinterpret_cast<const uint4*>(h + 4);
     }
 }
 
+// one piece of a side as the output wants it
 template <bool Q8, bool HALF_OUT>
-__global__ void __launch_bounds__(256) kv_read_kernel(const KvRowsArgs A) {
-    pdl_wait_then_release();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const bool side = blockIdx.y != 0;
-    void* out = side ? A.v_out : A.k_out;
-    if (i >= A.total || !out) return;
-    const int row = (int)(i / A.chunks), col = (int)(i - (long long)row * A.chunks);
-    const int seq = A.seq[row];
-    if (seq < 0) return;
-    const KvSlot at = kv_slot(A.table, A.n_seqs, A.max_pages, A.c.page_tokens, A.c.n_pages, seq, A.pos[row]);
-    if (at.page < 0) {
-        *(volatile int*)A.status = FQ_ERR_PAGE;
-        return;
-    }
-    size_t elem, sc;
-    piece_offsets(A.c, at, col, elem, sc);
-    const uint8_t* in = side ? A.c.v : A.c.k;
-    const size_t o = (size_t)i * 8;
+__device__ __forceinline__ void write_piece(const uint4& raw, float s, void* out, size_t o) {
     if (!Q8 && HALF_OUT) {
-        *reinterpret_cast<uint4*>((__half*)out + o) = ldg_stream16(in + elem * 2);
+        *reinterpret_cast<uint4*>((__half*)out + o) = raw;
         return;
     }
     float f[8];
     if (Q8) {
-        const uint2 raw = *reinterpret_cast<const uint2*>(in + elem);
-        const float s = __half2float((side ? A.c.v_scale : A.c.k_scale)[sc]);
         const int8_t* q = reinterpret_cast<const int8_t*>(&raw);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = (float)q[j] * s;  // 19 bits: exact in f32
     } else {
-        const uint4 raw = ldg_stream16(in + elem * 2);
         const __half2* h = reinterpret_cast<const __half2*>(&raw);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -164,12 +151,59 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvRowsArgs A) {
     }
 }
 
+template <bool Q8, bool HALF_OUT>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRowsArgs A) {
+    pdl_wait_then_release();
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= A.total) return;
+    const unsigned row = A.pieces.div(i), col = i - row * A.pieces.d;
+    const int seq = A.seq[row];
+    if (seq < 0) return;
+    const KvSlot at = kv_slot(A.table, A.n_seqs, A.max_pages, A.page_tokens, A.c.n_pages, seq, A.pos[row]);
+    if (at.page < 0) {
+        *(volatile int*)A.status = FQ_ERR_PAGE;
+        return;
+    }
+    size_t elem, sc;
+    piece_offsets(A, at, col, elem, sc);
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    float ks = 0.0f, vs = 0.0f;
+    if (Q8) {
+        if (A.k_out) {
+            const uint2 x = *reinterpret_cast<const uint2*>(A.c.k + elem);
+            k.x = x.x, k.y = x.y, ks = __half2float(A.c.k_scale[sc]);
+        }
+        if (A.v_out) {
+            const uint2 x = *reinterpret_cast<const uint2*>(A.c.v + elem);
+            v.x = x.x, v.y = x.y, vs = __half2float(A.c.v_scale[sc]);
+        }
+    } else {
+        if (A.k_out) k = *reinterpret_cast<const uint4*>(A.c.k + elem * 2);
+        if (A.v_out) v = *reinterpret_cast<const uint4*>(A.c.v + elem * 2);
+    }
+    const size_t o = (size_t)i * 8;
+    if (A.k_out) write_piece<Q8, HALF_OUT>(k, ks, A.k_out, o);
+    if (A.v_out) write_piece<Q8, HALF_OUT>(v, vs, A.v_out, o);
+}
+
 int check_rows(const KvView& c, const int32_t* seq, const int32_t* pos, size_t n_tokens, const int32_t* table, size_t n_seqs, size_t max_pages) {
     if (!seq || !pos || !table) return fail(FQ_DECLINED_ARGS, "null pointer");
     if (n_seqs == 0 || n_seqs > (size_t)INT32_MAX || max_pages == 0 || max_pages > (size_t)INT32_MAX / c.page_tokens)
         return fail(FQ_DECLINED_ARGS, "page table of %zu x %zu entries", n_seqs, max_pages);
-    if (n_tokens > ((size_t)1 << 38) / ((size_t)c.kv_heads * c.d)) return fail(FQ_DECLINED_ARGS, "more than 2^38 values in one call");
+    if (n_tokens > ((size_t)1 << 33) / ((size_t)c.kv_heads * c.d)) return fail(FQ_DECLINED_ARGS, "more than 2^33 values in one call");
     return FQ_OK;
+}
+
+// (total is below 2^30: check_rows)
+KvRowsArgs rows_args(const KvView& c, const int32_t* seq, const int32_t* pos, size_t n_tokens, const int32_t* table, size_t n_seqs,
+                     size_t max_pages, int* status) {
+    KvRowsArgs a{};
+    const unsigned pieces = (unsigned)(c.kv_heads * c.d / 8);
+    a.c = c, a.seq = seq, a.pos = pos, a.table = table, a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages;
+    a.total = (unsigned)n_tokens * pieces;
+    a.pieces = FastDiv(pieces), a.head = FastDiv((unsigned)c.d / 8), a.page_tokens = FastDiv((unsigned)c.page_tokens);
+    a.status = status;
+    return a;
 }
 
 }  // namespace
@@ -195,9 +229,9 @@ int fq_kv_append_dev(const fq_kv_pages* pages, const float* k_dev, const float* 
     if (!ctx) return FQ_DECLINED_NO_GPU;
     std::lock_guard<std::recursive_mutex> g(g_dispatch_lock);
     g_trace.calls++;
-    KvRowsArgs a{c, k_dev, v_dev, row_stride, nullptr, nullptr, token_seq_dev, token_pos_dev, page_table_dev, (int)n_seqs, (int)max_pages,
-                (int)(width / 8), (long long)(n_tokens * (width / 8)), ctx->status_dev};
-    const dim3 grid((unsigned)((a.total + 255) / 256), 2);
+    KvRowsArgs a = rows_args(c, token_seq_dev, token_pos_dev, n_tokens, page_table_dev, n_seqs, max_pages, ctx->status_dev);
+    a.k_in = k_dev, a.v_in = v_dev, a.row_stride = row_stride;
+    const dim3 grid((a.total + 255) / 256);
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     const cudaError_t e = pages->fmt == FQ_KV_Q8_0 ? launch_pdl(kv_append_kernel<true>, grid, dim3(256), 0, st, a)
                                                    : launch_pdl(kv_append_kernel<false>, grid, dim3(256), 0, st, a);
@@ -218,10 +252,9 @@ int fq_kv_read_dev(const fq_kv_pages* pages, void* k_out_dev, void* v_out_dev, i
     if (!ctx) return FQ_DECLINED_NO_GPU;
     std::lock_guard<std::recursive_mutex> g(g_dispatch_lock);
     g_trace.calls++;
-    const int chunks = c.kv_heads * c.d / 8;
-    KvRowsArgs a{c, nullptr, nullptr, 0, k_out_dev, v_out_dev, token_seq_dev, token_pos_dev, page_table_dev, (int)n_seqs, (int)max_pages,
-                chunks, (long long)(n_tokens * (size_t)chunks), ctx->status_dev};
-    const dim3 grid((unsigned)((a.total + 255) / 256), 2);
+    KvRowsArgs a = rows_args(c, token_seq_dev, token_pos_dev, n_tokens, page_table_dev, n_seqs, max_pages, ctx->status_dev);
+    a.k_out = k_out_dev, a.v_out = v_out_dev;
+    const dim3 grid((a.total + 255) / 256);
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     const bool q8 = pages->fmt == FQ_KV_Q8_0;
     const cudaError_t e = q8 ? (out_is_f16 ? launch_pdl(kv_read_kernel<true, true>, grid, dim3(256), 0, st, a)

@@ -10,6 +10,12 @@
 // one serves the layers that balance their experts by a bias. Keys are 64-bit: among 256 experts two keys lie within
 // f32 rounding of each other about once in ten thousand tokens, and a router that then picks by rounding does not
 // reproduce.
+//
+// Bound: latency for a token, instruction issue for a batch (the logits are 4 bytes per 30 instructions). So a row is first
+// ranked on f32 keys whose error has a bound, in registers, a contiguous run of experts per lane; where the ranks'
+// neighbours lie further apart than twice the bound the 64-bit order is the same, and 64-bit arithmetic is needed for the
+// chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys in shared
+// memory.
 #include "internal.h"
 #include "runtime.h"
 
@@ -53,42 +59,57 @@ __device__ __forceinline__ void warp_best(unsigned long long& v, int& i) {
     }
 }
 
-// a warp per row; shared memory: the row's ordered keys
-__global__ void router_groups_kernel(const RouterArgs A) {
-    extern __shared__ unsigned long long router_smem[];
-    pdl_wait_then_release();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int row = blockIdx.x * warps + warp;
-    if (row >= A.rows) return;  // whole warps leave together
-    unsigned long long* key = router_smem + (size_t)warp * A.experts;
-    const float* x = A.logits + (size_t)row * A.experts;
-
-    float mx = -INFINITY;
-    double inv = 1.0;
-    if (!A.sigmoid) {
-        for (int e = lane; e < A.experts; e += 32) mx = fmaxf(mx, x[e]);  // a NaN never wins
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    auto raw = [&](float v) -> double {  // the score before the division by the softmax sum; 0 for a closed expert
+// A row's 64-bit scores: what a warp needs to turn a logit into one.
+struct Scores {
+    bool sigmoid;
+    float mx;      // softmax: the largest logit
+    double total;  // softmax: the sum of exp(x - mx)
+    // before the division by the softmax sum; 0 for a closed expert
+    __device__ __forceinline__ double raw(float v) const {
         if (v != v || v == -INFINITY) return 0.0;
-        if (A.sigmoid) return 1.0 / (1.0 + exp(-(double)v));
+        if (sigmoid) return 1.0 / (1.0 + exp(-(double)v));
         return v == mx ? 1.0 : exp((double)v - (double)mx);
-    };
-    if (!A.sigmoid) {
-        double sum = 0.0;
-        for (int e = lane; e < A.experts; e += 32) sum += raw(x[e]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
-        inv = sum > 0.0 ? sum : 1.0;
     }
+};
+
+// The largest logit and, for a softmax, the 64-bit sum.
+__device__ __forceinline__ Scores row_scores(const RouterArgs& A, const float* x, int lane) {
+    Scores r{A.sigmoid != 0, -INFINITY, 1.0};
+    if (A.sigmoid) return r;
+    for (int e = lane; e < A.experts; e += 32) r.mx = fmaxf(r.mx, x[e]);  // a NaN never wins
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) r.mx = fmaxf(r.mx, __shfl_xor_sync(0xffffffffu, r.mx, o));
+    double sum = 0.0;
+    for (int e = lane; e < A.experts; e += 32) sum += r.raw(x[e]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
+    r.total = sum > 0.0 ? sum : 1.0;
+    return r;
+}
+
+// Weights of the chosen experts (lane s holds slot s and its score) and the row's results.
+__device__ __forceinline__ void write_row(const RouterArgs& A, int row, int lane, int sel, double w) {
+    if (A.normalize) {
+        double total = 0.0;
+        for (int s = 0; s < A.k; ++s) total += __shfl_sync(0xffffffffu, w, s);
+        if (total > 0.0) w /= total;
+    }
+    if (lane < A.k) {
+        A.selected[(size_t)row * A.k + lane] = sel;
+        A.weights[(size_t)row * A.k + lane] = (float)(w * (double)A.scale);
+    }
+}
+
+// A row ranked on 64-bit keys, held in shared memory.
+__device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int lane, unsigned long long* key) {
+    const float* x = A.logits + (size_t)row * A.experts;
+    const Scores sc = row_scores(A, x, lane);
     for (int e = lane; e < A.experts; e += 32) {
         const float v = x[e];
         const bool closed = v != v || v == -INFINITY;
-        key[e] = closed ? kClosed : ordered(raw(v) / inv + (A.bias ? (double)A.bias[e] : 0.0));
+        key[e] = closed ? kClosed : ordered(sc.raw(v) / sc.total + (A.bias ? (double)A.bias[e] : 0.0));
     }
     __syncwarp();
-
     if (A.groups > 1) {
         const int size = A.experts / A.groups;
         unsigned long long rank[kMaxGroups / 32];
@@ -132,19 +153,171 @@ __global__ void router_groups_kernel(const RouterArgs A) {
         for (int e = lane; e < A.experts; e += 32)
             if (key[e] > bv) bv = key[e], bi = e;
         warp_best(bv, bi);
-        if (lane == s) sel_mine = bi, w_mine = raw(x[bi]) / inv;
+        if (lane == s) sel_mine = bi, w_mine = sc.raw(x[bi]) / sc.total;
         __syncwarp();
         if (lane == 0) key[bi] = kTaken;
         __syncwarp();
     }
-    if (A.normalize) {
-        double total = 0.0;
-        for (int s = 0; s < A.k; ++s) total += __shfl_sync(0xffffffffu, w_mine, s);
-        if (total > 0.0) w_mine /= total;
-    }
-    if (lane < A.k) {
-        A.selected[(size_t)row * A.k + lane] = sel_mine;
-        A.weights[(size_t)row * A.k + lane] = (float)(w_mine * (double)A.scale);
+    write_row(A, row, lane, sel_mine, w_mine);
+}
+
+// f32 keys as unsigned integers in key order; 0: taken or closed
+__device__ __forceinline__ unsigned ordered32(float key) {
+    const unsigned b = __float_as_uint(key + 0.0f);
+    return b ^ ((int)b < 0 ? ~0u : 0x80000000u);
+}
+__device__ __forceinline__ float key_of32(unsigned u) { return __uint_as_float(u ^ (u >> 31 ? 0x80000000u : ~0u)); }
+
+// One round of a ranking over the warp's values, one per lane (0: none): the lane that holds the largest, or -1 where doubt
+// remains: it is less than `apart` below the one before, or two lanes hold it, or it is no number. -2: none is left.
+__device__ __forceinline__ int next_best(unsigned mine, float apart, float& prev) {
+    const unsigned top = __reduce_max_sync(0xffffffffu, mine);
+    if (top == 0) return -2;
+    const float v = key_of32(top);
+    const unsigned who = __ballot_sync(0xffffffffu, mine == top);
+    if (!(prev - v > apart) || (who & (who - 1)) || !(fabsf(v) < INFINITY)) return -1;
+    prev = v;
+    return __ffs(who) - 1;
+}
+
+// NE consecutive experts per lane (NE = 0: every row on 64-bit keys); groups are whole lanes, 2^n of them, or absent.
+// A warp per row.
+template <int NE>
+__global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constant__ RouterArgs A) {
+    extern __shared__ unsigned long long router_smem[];
+    pdl_wait_then_release();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int row = blockIdx.x * warps + warp;
+    if (row >= A.rows) return;  // whole warps leave together
+    unsigned long long* smem = router_smem + (size_t)warp * A.experts;
+    if constexpr (NE == 0) {
+        route_row_exact(A, row, lane, smem);
+    } else {
+        const float* x = A.logits + (size_t)row * A.experts;
+        float v[NE];
+#pragma unroll
+        for (int j = 0; j < NE; ++j) v[j] = lane * NE + j < A.experts ? x[lane * NE + j] : -INFINITY;
+        unsigned key[NE];
+        float apart, mx = 0.0f;
+        bool sure = true;
+        const bool sums = A.groups > 1 && A.top2 && A.experts > A.groups;  // ranks add two keys
+        // keys and twice the bound of their error. sigmoid: exp2 and the reciprocal are off by some 2^-22 each, the product in the
+        // exponent by |x| 2^-23 where the score falls as e^-|x|: below 2^-20 together, the addition of the bias by 2^-24 of the key.
+        // softmax without a bias: the logits themselves, exact; what lies e^-700 below the largest, or 1e-9 from a neighbour, is
+        // left to 64 bits, where such scores may coincide. softmax with a bias, or where scores are added: below 4e-6 (exp2 2^-22,
+        // the exponent's rounding |x - max| 2^-23 e^-|x - max|, at most 21 additions of the sum 2^-24 each, the division).
+        if (A.sigmoid) {
+            float big = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NE; ++j) {
+                const int e = lane * NE + j;
+                const bool closed = !(v[j] > -INFINITY);  // NaN too
+                const float s = __fdividef(1.0f, 1.0f + __expf(-fmaxf(v[j], -80.0f)));
+                const float k = A.bias && e < A.experts ? s + A.bias[e] : s;
+                key[j] = closed ? 0u : ordered32(k);
+                if (!closed) big = fmaxf(big, fabsf(k));
+            }
+            big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+            apart = 2.0f * (9.6e-7f + big * 1.2e-7f);
+        } else {
+            mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NE; ++j) mx = fmaxf(mx, v[j]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (A.bias || sums) {
+                float p[NE], sum = 0.0f, big = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NE; ++j) p[j] = v[j] > -INFINITY ? __expf(v[j] - mx) : 0.0f, sum += p[j];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float inv = 1.0f / sum;
+#pragma unroll
+                for (int j = 0; j < NE; ++j) {
+                    const int e = lane * NE + j;
+                    const float k = A.bias && e < A.experts ? p[j] * inv + A.bias[e] : p[j] * inv;
+                    key[j] = v[j] > -INFINITY ? ordered32(k) : 0u;
+                    if (v[j] > -INFINITY) big = fmaxf(big, fabsf(k));
+                }
+                big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+                apart = 2.0f * (4e-6f + big * 1.2e-7f);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NE; ++j) key[j] = v[j] > -INFINITY && v[j] - mx > -700.0f ? ordered32(v[j]) : 0u;
+                apart = 1e-9f;
+            }
+        }
+        if (A.groups > 1) {
+            // the two best of the lane, then of the group's lanes (a run of 2^n); ranks of closed groups stay in doubt
+            const int lanes = A.experts / A.groups / NE;
+            float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NE; ++j) {
+                const float k = key[j] ? key_of32(key[j]) : -INFINITY;
+                if (k > a) b = a, a = k;
+                else if (k > b) b = k;
+            }
+            for (int o = 1; o < lanes; o <<= 1) {
+                const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+                b = fmaxf(fminf(a, oa), fmaxf(b, ob)), a = fmaxf(a, oa);
+            }
+            const bool leader = lane % lanes == 0 && lane * NE < A.experts;
+            const float rank = sums ? a + b : a;
+            unsigned mine = leader && rank > -INFINITY ? ordered32(rank) : 0u;
+            unsigned open = 0;  // lanes of open groups
+            const float far = mine && sums ? 2.0f * apart + 2.4e-7f * (fabsf(a) + fabsf(b)) : apart;
+            const float apart_ranks = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(far)));
+            float prev = INFINITY;
+            for (int r = 0; r < A.kept + (A.kept < A.groups); ++r) {
+                const int who = next_best(mine, apart_ranks, prev);
+                if (who < 0) {
+                    sure = sure && who == -2 && r == A.kept;
+                    break;
+                }
+                if (r < A.kept) {
+                    open |= (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << who;
+                    if (lane == who) mine = 0u;
+                }
+            }
+            if (!((open >> lane) & 1)) {
+#pragma unroll
+                for (int j = 0; j < NE; ++j) key[j] = 0u;
+            }
+        }
+        int sel_mine = 0;
+        float v_mine = 0.0f;
+        if (sure) {
+            float prev = INFINITY;
+            for (int r = 0; r <= A.k; ++r) {  // the first one not taken included
+                unsigned top = key[0];
+                int at = 0;
+                float xv = v[0];
+#pragma unroll
+                for (int j = 1; j < NE; ++j)
+                    if (key[j] > top) top = key[j], at = j, xv = v[j];
+                // equal keys inside a lane: the second one shows in the next round, no distance apart
+                const int who = next_best(top, apart, prev);
+                if (who < 0) {
+                    sure = who == -2 && r == A.k;
+                    break;
+                }
+                const int e = __shfl_sync(0xffffffffu, lane * NE + at, who);
+                xv = __shfl_sync(0xffffffffu, xv, who);
+                if (lane == r && r < A.k) sel_mine = e, v_mine = xv;
+                if (lane == who) {
+#pragma unroll
+                    for (int j = 0; j < NE; ++j)
+                        if (j == at) key[j] = 0u;
+                }
+            }
+        }
+        if (!sure) {
+            route_row_exact(A, row, lane, smem);
+            return;
+        }
+        Scores sc{A.sigmoid != 0, mx, 1.0};
+        if (!A.sigmoid && !A.normalize) sc = row_scores(A, x, lane);  // normalised weights do not need the sum of all
+        write_row(A, row, lane, sel_mine, lane < A.k ? sc.raw(v_mine) / sc.total : 0.0);
     }
 }
 
@@ -173,8 +346,20 @@ extern "C" int fq_router_groups_dev(const float* logits_dev, size_t seq, size_t 
     const RouterArgs a{logits_dev, bias_dev, (int)seq, (int)n_expert, (int)top_k, score == FQ_SCORE_SIGMOID, (int)n_group, (int)topk_group,
                        group_score == FQ_GROUP_TOP2, normalize != 0, scale, selected_dev, weights_dev};
     const int warps = n_expert <= 1024 ? 4 : 1;  // eight bytes of shared memory per expert and warp, 32 KB at most
-    const cudaError_t e = launch_pdl(router_groups_kernel, dim3((unsigned)((seq + warps - 1) / warps)), dim3(warps * 32),
-                                     sizeof(unsigned long long) * n_expert * warps, st, a);
+    const dim3 grid((unsigned)((seq + warps - 1) / warps)), block(warps * 32);
+    const size_t smem = sizeof(unsigned long long) * n_expert * warps;
+    // experts per lane: the fewest that cover the row with every group on 2^n whole lanes
+    auto fits = [&](size_t ne) {
+        if (32 * ne < n_expert) return false;
+        const size_t size = n_expert / n_group, lanes = size / ne;
+        return n_group == 1 || (size % ne == 0 && (lanes & (lanes - 1)) == 0);
+    };
+    cudaError_t e;
+    if (fits(2)) e = launch_pdl(router_groups_kernel<2>, grid, block, smem, st, a);
+    else if (fits(4)) e = launch_pdl(router_groups_kernel<4>, grid, block, smem, st, a);
+    else if (fits(8)) e = launch_pdl(router_groups_kernel<8>, grid, block, smem, st, a);
+    else if (fits(16)) e = launch_pdl(router_groups_kernel<16>, grid, block, smem, st, a);
+    else e = launch_pdl(router_groups_kernel<0>, grid, block, smem, st, a);
     g_trace.launches++;
     return e == cudaSuccess ? FQ_OK : cuda_fail(e, "router launch");
 }

@@ -63,6 +63,14 @@ def _vp(x) -> C.c_void_p:
     raise TypeError(type(x))
 
 
+def _addr(x):
+    """`_vp` for entries called every token: the address itself, which ctypes converts by the declared argument type."""
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return x if x is None or isinstance(x, int) else _vp(x)
+
+
 def init(device: int = -1) -> None:
     _check(load().fq_init(device))
 
@@ -215,15 +223,19 @@ class KvPages:
 def kv_append_dev(pages: KvPages, k_dev, v_dev, token_seq_dev, token_pos_dev, n_tokens: int, page_table_dev, n_seqs: int, max_pages: int,
                   row_stride: int = 0, stream: int = 0) -> None:
     """Rows of f32 keys and values into their pages (`fq_kv_append_dev`); rows with token_seq < 0 are skipped."""
-    _check(load().fq_kv_append_dev(pages.ref, _vp(k_dev), _vp(v_dev), row_stride, _vp(token_seq_dev), _vp(token_pos_dev), n_tokens,
-                                   _vp(page_table_dev), n_seqs, max_pages, C.c_void_p(stream)))
+    rc = load().fq_kv_append_dev(pages.ref, _addr(k_dev), _addr(v_dev), row_stride, _addr(token_seq_dev), _addr(token_pos_dev), n_tokens,
+                                 _addr(page_table_dev), n_seqs, max_pages, stream)
+    if rc:
+        _check(rc)
 
 
 def kv_read_dev(pages: KvPages, k_out_dev, v_out_dev, out_is_f16: bool, token_seq_dev, token_pos_dev, n_tokens: int, page_table_dev,
                 n_seqs: int, max_pages: int, stream: int = 0) -> None:
     """Rows of the cache as dense f32 or f16 rows (`fq_kv_read_dev`), the K and V operands of `attn_fwd_dev`."""
-    _check(load().fq_kv_read_dev(pages.ref, _vp(k_out_dev), _vp(v_out_dev), int(out_is_f16), _vp(token_seq_dev), _vp(token_pos_dev), n_tokens,
-                                 _vp(page_table_dev), n_seqs, max_pages, C.c_void_p(stream)))
+    rc = load().fq_kv_read_dev(pages.ref, _addr(k_out_dev), _addr(v_out_dev), int(out_is_f16), _addr(token_seq_dev), _addr(token_pos_dev), n_tokens,
+                               _addr(page_table_dev), n_seqs, max_pages, stream)
+    if rc:
+        _check(rc)
 
 
 def attn_paged_workspace_bytes(pages: KvPages, n_seqs: int, heads: int, max_len: int) -> int:
@@ -235,8 +247,10 @@ def attn_paged_dev(pages: KvPages, q_dev, out_dev, page_table_dev, kv_len_dev, n
                    window: int = 0, max_len: int = 0, q_stride: int = 0, stats_dev=None, workspace=None, workspace_bytes: int = 0,
                    stream: int = 0) -> None:
     """Attention of one new token per sequence over its pages (`fq_attn_paged_dev`): q, out [n_seqs][heads][d] f32."""
-    _check(load().fq_attn_paged_dev(pages.ref, _vp(q_dev), q_stride, _vp(page_table_dev), _vp(kv_len_dev), n_seqs, max_pages, max_len, heads,
-                                    scale, window, _vp(out_dev), _vp(stats_dev), _vp(workspace), workspace_bytes, C.c_void_p(stream)))
+    rc = load().fq_attn_paged_dev(pages.ref, _addr(q_dev), q_stride, _addr(page_table_dev), _addr(kv_len_dev), n_seqs, max_pages, max_len, heads,
+                                  scale, window, _addr(out_dev), _addr(stats_dev), _addr(workspace), workspace_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 class _GgufTensor(C.Structure):
@@ -639,8 +653,10 @@ def router_groups_dev(logits_dev, seq: int, n_expert: int, top_k: int, selected_
                       n_group: int = 1, topk_group: int = 1, group_score: int = GROUP_MAX, normalize: bool = True, scale: float = 1.0,
                       stream: int = 0) -> None:
     """Expert choice by softmax or sigmoid scores with a balance bias and expert groups (`fq_router_groups_dev`)."""
-    _check(load().fq_router_groups_dev(_vp(logits_dev), seq, n_expert, score, _vp(bias_dev), n_group, topk_group, group_score, top_k,
-                                       int(normalize), scale, _vp(selected_dev), _vp(weights_dev), C.c_void_p(stream)))
+    rc = load().fq_router_groups_dev(_addr(logits_dev), seq, n_expert, score, _addr(bias_dev), n_group, topk_group, group_score, top_k,
+                                     int(normalize), scale, _addr(selected_dev), _addr(weights_dev), stream)
+    if rc:
+        _check(rc)
 
 
 # --------------------------------------------------------------------------- gates

@@ -190,7 +190,7 @@ typedef struct {
 /* Write n_tokens rows of keys and values: row r is position token_pos[r] of sequence token_seq[r]; rows with
  * token_seq < 0 (padding) are skipped. k_dev and v_dev are f32 [n_tokens][kv_heads * d] with row_stride elements
  * between rows (0 = dense; a multiple of 4), so both may point into the rows of a fused projection. No two rows of a
- * call may name the same slot. n_tokens 0 does nothing. Neither allocates nor synchronises. */
+ * call may name the same slot. n_tokens 0 does nothing; n_tokens * kv_heads * d <= 2^33. Neither allocates nor synchronises. */
 FQ_API int fq_kv_append_dev(const fq_kv_pages* pages, const float* k_dev, const float* v_dev, size_t row_stride,
                             const int32_t* token_seq_dev, const int32_t* token_pos_dev, size_t n_tokens, const int32_t* page_table_dev,
                             size_t n_seqs, size_t max_pages, void* stream);
