@@ -14,8 +14,8 @@
 // Bound: latency for a token, instruction issue for a batch (the logits are 4 bytes per 30 instructions). So a row is first
 // ranked on f32 keys whose error has a bound, in registers, a contiguous run of experts per lane; where the ranks'
 // neighbours lie further apart than twice the bound the 64-bit order is the same, and 64-bit arithmetic is needed for the
-// chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys in shared
-// memory.
+// chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys. Rows whose
+// groups do not fall on whole lanes, or of more than 512 experts, are ranked on 64-bit keys in shared memory at once.
 #include "internal.h"
 #include "runtime.h"
 
@@ -161,6 +161,99 @@ __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int la
     write_row(A, row, lane, sel_mine, w_mine);
 }
 
+// The lane that holds the warp's largest value (0: none), the lowest of several: by the upper halves, then the lower ones.
+__device__ __forceinline__ int best_lane(unsigned long long mine) {
+    const unsigned hi = (unsigned)(mine >> 32), top = __reduce_max_sync(0xffffffffu, hi);
+    unsigned who = __ballot_sync(0xffffffffu, hi == top);
+    if (who & (who - 1)) {
+        const unsigned lo = hi == top ? (unsigned)mine : 0u, top_lo = __reduce_max_sync(0xffffffffu, lo);
+        who = __ballot_sync(0xffffffffu, hi == top && lo == top_lo);
+    }
+    return __ffs(who) - 1;
+}
+
+// The same for NE consecutive experts per lane, in registers (experts v, groups of whole lanes).
+template <int NE>
+__device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int lane) {
+    const float* x = A.logits + (size_t)row * A.experts;
+    Scores sc{A.sigmoid != 0, -INFINITY, 1.0};
+    float v[NE];
+    double p[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) v[j] = lane * NE + j < A.experts ? x[lane * NE + j] : -INFINITY;
+    if (!A.sigmoid) {
+#pragma unroll
+        for (int j = 0; j < NE; ++j) sc.mx = fmaxf(sc.mx, v[j]);  // a NaN never wins
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sc.mx = fmaxf(sc.mx, __shfl_xor_sync(0xffffffffu, sc.mx, o));
+    }
+#pragma unroll
+    for (int j = 0; j < NE; ++j) p[j] = sc.raw(v[j]);
+    if (!A.sigmoid) {
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) sum += p[j];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += shfl_xor_d(sum, o);
+        sc.total = sum > 0.0 ? sum : 1.0;
+    }
+    unsigned long long key[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+        const int e = lane * NE + j;
+        if (!A.sigmoid) p[j] /= sc.total;
+        const bool closed = !(v[j] > -INFINITY);
+        key[j] = e >= A.experts ? kTaken : closed ? kClosed : ordered(p[j] + (A.bias ? (double)A.bias[e] : 0.0));
+    }
+    if (A.groups > 1) {
+        const int size = A.experts / A.groups, lanes = size / NE;
+        unsigned long long a = 0, b = 0;  // the two largest of the lane, then of the group's lanes
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+            if (key[j] > a) b = a, a = key[j];
+            else if (key[j] > b) b = key[j];
+        }
+        for (int o = 1; o < lanes; o <<= 1) {
+            const unsigned long long oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+            const unsigned long long low = a < oa ? a : oa, second = b > ob ? b : ob;
+            b = low > second ? low : second, a = a > oa ? a : oa;
+        }
+        const bool leader = lane % lanes == 0 && lane * NE < A.experts;
+        unsigned long long rank = !leader ? kTaken : A.top2 && size > 1 ? ordered(key_of(a) + key_of(b)) : a;
+        unsigned open = 0;
+        for (int r = 0; r < A.kept; ++r) {
+            const int who = best_lane(rank);
+            open |= (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << who;
+            if (lane == who) rank = kTaken;
+        }
+        if (!((open >> lane) & 1)) {
+#pragma unroll
+            for (int j = 0; j < NE; ++j)
+                if (key[j] != kTaken) key[j] = kClosed;
+        }
+    }
+    double w_mine = 0.0;
+    int sel_mine = 0;
+    for (int s = 0; s < A.k; ++s) {
+        unsigned long long top = key[0];
+        int at = 0;
+        double pv = p[0];
+#pragma unroll
+        for (int j = 1; j < NE; ++j)
+            if (key[j] > top) top = key[j], at = j, pv = p[j];
+        const int who = best_lane(top);
+        const int e = __shfl_sync(0xffffffffu, lane * NE + at, who);
+        pv = __shfl_sync(0xffffffffu, pv, who);
+        if (lane == s) sel_mine = e, w_mine = pv;
+        if (lane == who) {
+#pragma unroll
+            for (int j = 0; j < NE; ++j)
+                if (j == at) key[j] = kTaken;
+        }
+    }
+    write_row(A, row, lane, sel_mine, w_mine);
+}
+
 // f32 keys as unsigned integers in key order; 0: taken or closed
 __device__ __forceinline__ unsigned ordered32(float key) {
     const unsigned b = __float_as_uint(key + 0.0f);
@@ -189,9 +282,8 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int row = blockIdx.x * warps + warp;
     if (row >= A.rows) return;  // whole warps leave together
-    unsigned long long* smem = router_smem + (size_t)warp * A.experts;
     if constexpr (NE == 0) {
-        route_row_exact(A, row, lane, smem);
+        route_row_exact(A, row, lane, router_smem + (size_t)warp * A.experts);
     } else {
         const float* x = A.logits + (size_t)row * A.experts;
         float v[NE];
@@ -312,7 +404,7 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
             }
         }
         if (!sure) {
-            route_row_exact(A, row, lane, smem);
+            route_row_exact<NE>(A, row, lane);
             return;
         }
         Scores sc{A.sigmoid != 0, mx, 1.0};
@@ -347,7 +439,6 @@ extern "C" int fq_router_groups_dev(const float* logits_dev, size_t seq, size_t 
                        group_score == FQ_GROUP_TOP2, normalize != 0, scale, selected_dev, weights_dev};
     const int warps = n_expert <= 1024 ? 4 : 1;  // eight bytes of shared memory per expert and warp, 32 KB at most
     const dim3 grid((unsigned)((seq + warps - 1) / warps)), block(warps * 32);
-    const size_t smem = sizeof(unsigned long long) * n_expert * warps;
     // experts per lane: the fewest that cover the row with every group on 2^n whole lanes
     auto fits = [&](size_t ne) {
         if (32 * ne < n_expert) return false;
@@ -355,11 +446,11 @@ extern "C" int fq_router_groups_dev(const float* logits_dev, size_t seq, size_t 
         return n_group == 1 || (size % ne == 0 && (lanes & (lanes - 1)) == 0);
     };
     cudaError_t e;
-    if (fits(2)) e = launch_pdl(router_groups_kernel<2>, grid, block, smem, st, a);
-    else if (fits(4)) e = launch_pdl(router_groups_kernel<4>, grid, block, smem, st, a);
-    else if (fits(8)) e = launch_pdl(router_groups_kernel<8>, grid, block, smem, st, a);
-    else if (fits(16)) e = launch_pdl(router_groups_kernel<16>, grid, block, smem, st, a);
-    else e = launch_pdl(router_groups_kernel<0>, grid, block, smem, st, a);
+    if (fits(2)) e = launch_pdl(router_groups_kernel<2>, grid, block, 0, st, a);
+    else if (fits(4)) e = launch_pdl(router_groups_kernel<4>, grid, block, 0, st, a);
+    else if (fits(8)) e = launch_pdl(router_groups_kernel<8>, grid, block, 0, st, a);
+    else if (fits(16)) e = launch_pdl(router_groups_kernel<16>, grid, block, 0, st, a);
+    else e = launch_pdl(router_groups_kernel<0>, grid, block, sizeof(unsigned long long) * n_expert * warps, st, a);
     g_trace.launches++;
     return e == cudaSuccess ? FQ_OK : cuda_fail(e, "router launch");
 }
