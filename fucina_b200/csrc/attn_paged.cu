@@ -16,9 +16,9 @@
 // which ring walked what. Small calls have one chunk per ring. Large ones give each ring one chunk of three quarters of its
 // fair share and hand out the rest in small ones as rings become free: SMs differ by a fifth in the rate at which memory
 // serves them (64 f16 sequences of up to 8000 tokens: equal shares took 137 to 195 us per SM). A first kernel then adds up
-// the lengths and clears the hand-out counter. When every row is short, one CTA takes one row, its rings' pieces are joined
-// in shared memory, and that kernel is the only one. The lengths are read on the device: nothing on the host depends on
-// them.
+// the lengths and clears the hand-out counter. When every row is short, each row has a team of rings, some of a CTA's, all of
+// them, or those of a cluster of CTAs, as the number of rows leaves room; their pieces are joined in (distributed) shared
+// memory, and that kernel is the only one. The lengths are read on the device: nothing on the host depends on them.
 //
 // Copies. The keys of a stage are refilled as soon as the scores are taken, the values after the second product: nearly
 // two units per ring are in flight at any time from two stages' room.
@@ -29,6 +29,7 @@
 // rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's
 // smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a value's scale s turns the two parts
 // (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'), whose bracket is exact in f16.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -68,7 +69,8 @@ struct PagedArgs {
     int span;          // query heads of one row
     int warps_per_ring, heads_per_warp, rings;
     int stage_bytes;
-    int row_mode;      // one CTA per row
+    int row_mode;      // every row has a team of rings
+    int team, cluster; // its rings in a CTA, and CTAs
     int dynamic;       // the plan kernel has run: `sums` holds the units before each sequence, `next` counts handed-out chunks
     int min_units;     // per chunk
     unsigned page_magic;                  // index of 16 keys / 16-key runs of a page = umulhi(index, page_magic); 0: one run a page
@@ -282,12 +284,20 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         c.start_row(from - c.r * units);
     };
     cur = {0, 0, 1, 0, 0, 0};
+    // row_mode: this ring's row and place in the team
+    const int teams = A.rings / A.team;
     if (A.row_mode) {
-        cur.s = blockIdx.x / rows_per_seq, cur.r = blockIdx.x - cur.s * rows_per_seq;
-        key_range(A, cur.s, cur.first, cur.end);
-        const int units = cur.units(), u = units * ring / A.rings;  // a row of few units
-        count = units * (ring + 1) / A.rings - u;
-        cur.start_row(u);
+        const int in_cta = ring / A.team, row = blockIdx.x / A.cluster * teams + in_cta;
+        count = 0;
+        if (in_cta < teams && row < A.n_seqs * rows_per_seq) {
+            cur.s = row / rows_per_seq, cur.r = row - cur.s * rows_per_seq;
+            key_range(A, cur.s, cur.first, cur.end);
+            // a row of few units
+            const int units = cur.units(), rank = blockIdx.x % A.cluster * A.team + ring - in_cta * A.team, size = A.cluster * A.team;
+            const int u = units * rank / size;
+            count = units * (rank + 1) / size - u;
+            cur.start_row(u);
+        }
     } else {
         const int from = split.begin(chunk);
         count = split.begin(chunk + 1) - from;
@@ -306,6 +316,11 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         ++asked;
         to_post = true;
     };
+    auto post = [&]() {
+        if (!to_post) return;
+        if (part == 0 && lane == 0) sh_next[ring][(asked - 1) & 1] = answer;
+        to_post = false;
+    };
     if (dynamic && count > 0) ask(split.begin(chunk) + count);
 
     // ---- copies. `ahead` is the unit copied next; its pages are looked up a step before they are needed. A unit is one or two
@@ -318,7 +333,10 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     int coming_chunk = -1, coming_count = 0;
     unsigned have = 0;  // runs of the unit to copy that exist
     unsigned gone_new = 0, gone_next = 0, gone_now = 0;  // runs whose page is no page: of the unit to copy, and of the two in the stages
-    int pg[RUNS], pu[RUNS];
+    struct Look {
+        unsigned want;  // runs with keys in range
+        int pg[RUNS], at[RUNS];
+    };
     size_t run[RUNS], srun[RUNS];
     const int runs_per_page = A.c.page_tokens / kSub;
     const int* table = A.table;
@@ -327,32 +345,34 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         table = A.table + (size_t)ahead.s * A.max_pages;
         head_run = ahead.r / A.passes * runs_per_page;
     };
-    auto look_up = [&]() {
+    auto look_up = [&](Look& k) {
+        k.want = 0;
 #pragma unroll
         for (int x = 0; x < RUNS; ++x) {
             const int i = ahead.key / kSub + x;
-            pg[x] = -1;
+            k.pg[x] = -1, k.at[x] = 0;
             if (i * kSub < ahead.end && (i + 1) * kSub > ahead.first) {
                 const int slot = A.page_magic ? (int)__umulhi((unsigned)i, A.page_magic) : i;
-                pu[x] = head_run + i - slot * runs_per_page;
-                pg[x] = table[slot];
+                k.want |= 1u << x;
+                k.at[x] = head_run + i - slot * runs_per_page;
+                k.pg[x] = table[slot];
             }
         }
     };
     // after the look-up's loads have arrived
-    auto place = [&]() {
+    auto place = [&](const Look& k) {
         have = gone_new = 0;
 #pragma unroll
         for (int x = 0; x < RUNS; ++x) {
-            const int i = ahead.key / kSub + x;
-            if ((unsigned)pg[x] < (unsigned)A.c.n_pages) {
+            if ((unsigned)k.pg[x] < (unsigned)A.c.n_pages) {
                 have |= 1u << x;
-                run[x] = (size_t)(unsigned)pg[x] * A.page_chunks + (unsigned)(pu[x] * kSub * nc);
-                if (Q8) srun[x] = (size_t)(unsigned)pg[x] * A.scale_chunks + (unsigned)(pu[x] * nc);
-            } else if (i * kSub < ahead.end && (i + 1) * kSub > ahead.first) {
-                *(volatile int*)A.status = FQ_ERR_PAGE;
-                gone_new |= 1u << x;
+                run[x] = (size_t)(unsigned)k.pg[x] * A.page_chunks + (unsigned)(k.at[x] * kSub * nc);
+                if (Q8) srun[x] = (size_t)(unsigned)k.pg[x] * A.scale_chunks + (unsigned)(k.at[x] * nc);
             }
+        }
+        if (have != k.want) {
+            *(volatile int*)A.status = FQ_ERR_PAGE;
+            gone_new = have ^ k.want;
         }
     };
     const unsigned row_magic = (65536u + nc - 1) / nc;  // chunk / nc = chunk * row_magic >> 16 for chunks < 512
@@ -386,15 +406,13 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         }
         cp_async_commit();
     };
+    Look look;
     auto step_ahead = [&]() {
         gone_now = gone_next, gone_next = gone_new;
-        if (to_post) {
-            if (part == 0 && lane == 0) sh_next[ring][(asked - 1) & 1] = answer;
-            to_post = false;
-        }
+        post();
         if (--left > 0) {
             if (ahead.next(A, rows_per_seq)) enter_row();
-            look_up();
+            look_up(look);
         } else if (left == 0 && more) {
             const int c = sh_next[ring][(asked - 1) & 1];
             const int from = split.begin(c), n = split.begin(c + 1) - from;
@@ -405,17 +423,31 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                 left = n;
                 coming = ahead, coming_chunk = c, coming_count = n;
                 enter_row();
-                look_up();
+                look_up(look);
             }
         }
     };
-    if (count > 0) enter_row(), look_up();
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        if (left > 0) place();
-        copy_side(s * A.stage_bytes, 0);
-        copy_side(s * A.stage_bytes, 1);
-        step_ahead();
+    // the first two units, both looked up before either is waited for (more than two follow, or none)
+    {
+        Look first{0, {}, {}}, second{0, {}, {}};
+        if (count > 0) enter_row(), look_up(first);
+        if (count > 1) {
+            if (ahead.next(A, rows_per_seq)) enter_row();
+            look_up(second);
+        }
+        if (left > 0) place(first);
+        copy_side(0, 0);
+        copy_side(0, 1);
+        gone_now = gone_new;
+        if (--left > 0) place(second);
+        copy_side(A.stage_bytes, 0);
+        copy_side(A.stage_bytes, 1);
+        gone_next = gone_new, gone_new = 0;
+        post();  // a chunk of three units reads the answer in its first step, behind that step's barriers
+        if (left > 0 && --left > 0) {
+            if (ahead.next(A, rows_per_seq)) enter_row();
+            look_up(look);
+        }
     }
 
     // ---- the share, piece by piece
@@ -541,7 +573,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             for (int n = 0; n < NT; ++n) sc[n][0] = whole(c[n][0], c[n][2]), sc[n][1] = whole(c[n][1], c[n][3]);
         }
         ring_sync();  // all the ring's warps are done with the keys
-        if (left > 0) place();
+        if (left > 0) place(look);
         copy_side(stage_at, 0);
 
         // ---- weights
@@ -581,11 +613,14 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         if (partial) {
             // values that do not take part may be anything: their rows (Q8_0: their scales) become zeros. The ring's warps write
             // the same zeros.
-            uint8_t* rows = ring_base + stage_at + (Q8 ? v_scale_at : UK * pitch);
-            const int bytes = Q8 ? nb * 2 : d * 2, step = Q8 ? nb * 2 : pitch;
-            for (int r = 0; r < UK; ++r)
-                if (!takes_part(r))
-                    for (int i = lane * 2; i < bytes; i += 64) *reinterpret_cast<uint16_t*>(rows + r * step + i) = 0;
+            if (Q8) {
+                __half* rows = reinterpret_cast<__half*>(ring_base + stage_at + v_scale_at);
+                for (int i = lane; i < UK * nb; i += 32)
+                    if (!takes_part(i / nb)) rows[i] = __ushort_as_half(0);
+            } else {
+                for (int i = lane; i < UK * nc; i += 32)
+                    if (!takes_part(i / nc)) *reinterpret_cast<uint4*>(ring_base + stage_at + UK * pitch + (i + i / nc) * 16) = make_uint4(0, 0, 0, 0);
+            }
             __syncwarp();
         }
         if (Q8) {
@@ -713,50 +748,75 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     }
     if (!A.row_mode) return;
 
-    // ---- join the rings' pieces of this CTA's row, in order: a warp per head row, a lane per piece for the weights, then four
-    // values a lane. A row of one unit was finished by its ring.
-    __syncthreads();
-    const int s = blockIdx.x / rows_per_seq, r = blockIdx.x - s * rows_per_seq, kvh = r / A.passes;
-    int first, end;
-    key_range(A, s, first, end);
-    const int units = units_of<UK>(first, end), warps = blockDim.x >> 5;
-    if (units == 1 || A.rings == 1) return;
+    // ---- join the teams' pieces, in order: a warp per (row, head row), a lane per piece for the weights (two where a team has
+    // more than 32 rings), then four values a lane, eight pieces at a time
+    namespace cg = cooperative_groups;
+    if (A.cluster > 1) cg::this_cluster().sync();
+    else __syncthreads();
+    const int size = A.cluster * A.team, warps = blockDim.x >> 5, cta = blockIdx.x % A.cluster;
     const size_t ring_floats = (size_t)2 * A.stage_bytes / sizeof(float);
-    const float* pieces = reinterpret_cast<const float*>(smem);
-    const bool in = lane < A.rings && units * (lane + 1) / A.rings > units * lane / A.rings;
-    for (int pr = warp; pr < prow; pr += warps) {
+    for (int item = cta + A.cluster * warp; item < teams * prow && size > 1; item += A.cluster * warps) {
+        const int in_cta = item / prow, pr = item - in_cta * prow, row = blockIdx.x / A.cluster * teams + in_cta;
+        if (row >= A.n_seqs * rows_per_seq) continue;
+        const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
         const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
         if ((pr & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) continue;
-        float m = -INFINITY, l = 0.0f;
-        if (in) m = pieces[lane * ring_floats + prow * d + pr * 2], l = pieces[lane * ring_floats + prow * d + pr * 2 + 1];
-        float m_all = m;
+        int first, end;
+        key_range(A, s, first, end);
+        const int units = units_of<UK>(first, end);
+        if (units == 1) continue;  // finished by its ring
+        auto piece = [&](int k) {
+            const int c = k / A.team;
+            float* p = reinterpret_cast<float*>(smem) + (size_t)(in_cta * A.team + k - c * A.team) * ring_floats;
+            return A.cluster > 1 ? (const float*)cg::this_cluster().map_shared_rank(p, c) : (const float*)p;
+        };
+        float m[2], l[2], f[2], m_all = -INFINITY, l_all = 0.0f;
+        unsigned present[2];
 #pragma unroll
-        for (int x = kMaxRings / 2; x > 0; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
-        m_all = __shfl_sync(0xffffffffu, m_all, 0);
-        const float f = m == -INFINITY ? 0.0f : ex2((m - m_all) * kLog2e);
-        l = in ? l * f : 0.0f;
+        for (int x = 0; x < 2; ++x) {
+            const int k = lane + 32 * x;
+            const bool in = k < size && units * (k + 1) / size > units * k / size;
+            m[x] = -INFINITY, l[x] = 0.0f;
+            if (in) {
+                const float2 ml = *reinterpret_cast<const float2*>(piece(k) + (size_t)prow * d + pr * 2);
+                m[x] = ml.x, l[x] = ml.y;
+            }
+            present[x] = __ballot_sync(0xffffffffu, in);
+            m_all = fmaxf(m_all, m[x]);
+        }
 #pragma unroll
-        for (int x = kMaxRings / 2; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        l = __shfl_sync(0xffffffffu, l, 0);
+        for (int x = 16; x > 0; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            f[x] = m[x] == -INFINITY ? 0.0f : ex2((m[x] - m_all) * kLog2e);
+            l_all += l[x] * f[x];
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, x);
         const size_t at = (size_t)s * A.heads + (size_t)kvh * A.group + in_group;
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const unsigned present = __ballot_sync(0xffffffffu, in);
-#pragma unroll
-        for (int i0 = 0; i0 < DM; i0 += 128) {
+        const float inv = l_all > 0.0f || l_all != l_all ? 1.0f / l_all : 0.0f;
+        for (int i0 = 0; i0 < d; i0 += 128) {
             const int i = i0 + lane * 4;
             float4 a = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-            for (int e = 0; e < A.rings; ++e) {
-                const float fe = __shfl_sync(0xffffffffu, f, e);
-                if (i < d && ((present >> e) & 1)) {
-                    const float4 x = *reinterpret_cast<const float4*>(pieces + e * ring_floats + (size_t)pr * d + i);
-                    a.x = fmaf(x.x, fe, a.x), a.y = fmaf(x.y, fe, a.y), a.z = fmaf(x.z, fe, a.z), a.w = fmaf(x.w, fe, a.w);
+            for (int k0 = 0; k0 < size; k0 += 8) {
+                float4 v[8];
+                float fk[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int kk = k0 + k;
+                    const bool there = kk < size && ((kk < 32 ? present[0] >> kk : present[1] >> (kk - 32)) & 1);
+                    fk[k] = there ? __shfl_sync(0xffffffffu, kk < 32 ? f[0] : f[1], kk & 31) : 0.0f;
+                    v[k] = there && i < d ? *reinterpret_cast<const float4*>(piece(kk) + (size_t)pr * d + i) : make_float4(0, 0, 0, 0);
                 }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    a.x = fmaf(v[k].x, fk[k], a.x), a.y = fmaf(v[k].y, fk[k], a.y), a.z = fmaf(v[k].z, fk[k], a.z), a.w = fmaf(v[k].w, fk[k], a.w);
             }
             if (i < d) *reinterpret_cast<float4*>(A.out + at * d + i) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
         }
-        if (lane == 0 && A.stats) A.stats[at * 2] = l > 0.0f ? m_all : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
+        if (lane == 0 && A.stats) A.stats[at * 2] = l_all > 0.0f ? m_all : kNegBig, A.stats[at * 2 + 1] = l_all * (1.0f / 32768.0f);
     }
+    if (A.cluster > 1) cg::this_cluster().sync();  // no CTA leaves while another reads its pieces
 }
 
 // The units before each sequence, and a fresh hand-out counter: one CTA, 1024 sequences at a time.
@@ -925,13 +985,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 // How a call is cut, from sizes the host knows.
 struct Plan {
     int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
-    int row_mode, dynamic, grid, chunks;
+    int row_mode, team, cluster, dynamic, grid, chunks;
     size_t smem, sums_at, meta_at, parts_at, workspace;
 };
 
 // A chunk has at least two units (a ring's depth of copies; below that the joins cost more than the copies they spread),
 // three where chunks are handed out.
 constexpr int kMinUnits = 2, kMinUnitsDynamic = 3;
+
+// Teams walk rows of at most this many units per ring: longer ones are better spread over all rings.
+constexpr int kTeamUnits = 8;
 
 int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max_len, int sm_count, Plan* out) {
     Plan p;
@@ -948,16 +1011,22 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     // as many rings as warps and two stages each allow
     p.rings = max_warps(p.dm) / p.warps_per_ring;
     while (p.rings > 1 && p.rings * 2 * p.stage_bytes > kSmemMost) --p.rings;
-    if (p.rings * 2 * p.stage_bytes > kSmemMost || (size_t)2 * p.stage_bytes < piece)
-        return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
+    if (p.rings * 2 * p.stage_bytes > kSmemMost) return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
     p.smem = (size_t)p.rings * 2 * p.stage_bytes;
     const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / keys + 2;
     if (rows > (size_t)INT32_MAX / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
-    p.row_mode = units <= (size_t)4 * p.rings;
+    // Teams: the most rings per row with which all rows run at once; whole CTAs where that leaves half the SMs idle, up to a
+    // cluster of four (a team of 64 rings at most is joined by one warp).
+    p.team = p.rings, p.cluster = 1;
+    while (p.team > 1 && (rows + p.rings / p.team - 1) / (p.rings / p.team) > (size_t)sm_count) --p.team;
+    while (p.cluster < 4 && p.team == p.rings && 2 * rows * p.cluster <= (size_t)sm_count && units > (size_t)p.team * p.cluster) p.cluster *= 2;
+    // (a piece of a team lies on its ring's stages)
+    p.row_mode = units <= (size_t)kTeamUnits * p.team * p.cluster && (p.team * p.cluster == 1 || (size_t)2 * p.stage_bytes >= piece);
+    if (!p.row_mode) p.team = p.rings, p.cluster = 1;
     const size_t most = rows * units, rings_all = (size_t)sm_count * p.rings;
     p.dynamic = !p.row_mode && !q8 && most >= 48 * rings_all;
     const size_t shares = (most + kMinUnits - 1) / kMinUnits, ctas = (shares + p.rings - 1) / p.rings;
-    p.grid = p.row_mode ? (int)rows : (int)(ctas < (size_t)sm_count ? ctas : (size_t)sm_count);
+    p.grid = p.row_mode ? (int)((rows + p.rings / p.team - 1) / (p.rings / p.team)) * p.cluster : (int)(ctas < (size_t)sm_count ? ctas : (size_t)sm_count);
     // one chunk per ring; handed out, the rest (a quarter of the fair shares) in chunks of an eighth of one or of three units:
     // (fair / 4) / (fair / 8) rounded down is at most 5 / 1, and 3 where the least size binds
     p.chunks = p.grid * p.rings * (p.dynamic ? 6 : 1);
@@ -978,7 +1047,17 @@ cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         granted = true;
     }
-    return launch_pdl(attn_paged_kernel<Q8, DM, EXACT>, dim3((unsigned)p.grid), dim3((unsigned)(p.rings * p.warps_per_ring * 32)), p.smem, st, a);
+    const dim3 grid((unsigned)p.grid), block((unsigned)(p.rings * p.warps_per_ring * 32));
+    if (p.cluster == 1) return launch_pdl(attn_paged_kernel<Q8, DM, EXACT>, grid, block, p.smem, st, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = p.smem, cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = getenv("FUCINA_B200_NO_PDL") ? 1 : 2;
+    return cudaLaunchKernelEx(&cfg, attn_paged_kernel<Q8, DM, EXACT>, a);
 }
 template <bool Q8>
 cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
@@ -1057,7 +1136,7 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages, a.max_len = (int)max_len, a.heads = (int)heads, a.group = (int)heads / c.kv_heads;
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
     a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp;
-    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.dynamic = p.dynamic;
+    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.team = p.team, a.cluster = p.cluster, a.dynamic = p.dynamic;
     a.min_units = p.dynamic ? kMinUnitsDynamic : kMinUnits;
     const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
     a.page_magic = per_page == 1 ? 0 : (unsigned)(((1ull << 32) + per_page - 1) / per_page);  // exact below 2^32 / 256 runs of 16 keys

@@ -38,6 +38,8 @@ def run(P, kind, lens, page, heads, kv, d, window=0, seed=1, gain=1.0, max_len=0
     ([200, 90], 16, 9, 1, 32, 0),
     ([300, 40], 16, 80, 1, 64, 0),                  # eighty heads to a kv head
     ([260], 256, 6, 3, 160, 0),
+    ([180, 5], 16, 17, 1, 160, 0),                  # seventeen heads of 160
+    ([300, 290], 16, 31, 1, 192, 0),
     ([120, 300], 32, 4, 2, 256, 0),
     ([1000, 3, 40], 16, 8, 4, 128, 37),             # window starts inside a block of keys
     ([64, 65, 63], 16, 4, 4, 128, 64),
