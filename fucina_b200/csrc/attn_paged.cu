@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             const int u = units * rank / size;
             count = units * (rank + 1) / size - u;
             cur.start_row(u);
+            if (part == 0 && lane == 0) sh_next[ring][0] = units;  // for the join
         }
     } else {
         const int from = split.begin(chunk);
@@ -754,22 +755,18 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     if (A.cluster > 1) cg::this_cluster().sync();
     else __syncthreads();
     const int size = A.cluster * A.team, warps = blockDim.x >> 5, cta = blockIdx.x % A.cluster;
-    const size_t ring_floats = (size_t)2 * A.stage_bytes / sizeof(float);
+    const int ring_floats = 2 * A.stage_bytes / (int)sizeof(float);
     for (int item = cta + A.cluster * warp; item < teams * prow && size > 1; item += A.cluster * warps) {
         const int in_cta = item / prow, pr = item - in_cta * prow, row = blockIdx.x / A.cluster * teams + in_cta;
         if (row >= A.n_seqs * rows_per_seq) continue;
         const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
         const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
         if ((pr & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) continue;
-        int first, end;
-        key_range(A, s, first, end);
-        const int units = units_of<UK>(first, end);
+        const int units = sh_next[in_cta * A.team][0];
         if (units == 1) continue;  // finished by its ring
-        auto piece = [&](int k) {
-            const int c = k / A.team;
-            float* p = reinterpret_cast<float*>(smem) + (size_t)(in_cta * A.team + k - c * A.team) * ring_floats;
-            return A.cluster > 1 ? (const float*)cg::this_cluster().map_shared_rank(p, c) : (const float*)p;
-        };
+        // ring k of the team's part in CTA c
+        float* const here = reinterpret_cast<float*>(smem) + in_cta * A.team * ring_floats;
+        auto pieces_of = [&](int c) { return A.cluster > 1 ? (const float*)cg::this_cluster().map_shared_rank(here, c) : (const float*)here; };
         float m[2], l[2], f[2], m_all = -INFINITY, l_all = 0.0f;
         unsigned present[2];
 #pragma unroll
@@ -778,7 +775,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
             const bool in = k < size && units * (k + 1) / size > units * k / size;
             m[x] = -INFINITY, l[x] = 0.0f;
             if (in) {
-                const float2 ml = *reinterpret_cast<const float2*>(piece(k) + (size_t)prow * d + pr * 2);
+                const int c = A.cluster > 1 ? k / A.team : 0;
+                const float2 ml = *reinterpret_cast<const float2*>(pieces_of(c) + (k - c * A.team) * ring_floats + prow * d + pr * 2);
                 m[x] = ml.x, l[x] = ml.y;
             }
             present[x] = __ballot_sync(0xffffffffu, in);
@@ -798,19 +796,23 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         for (int i0 = 0; i0 < d; i0 += 128) {
             const int i = i0 + lane * 4;
             float4 a = make_float4(0, 0, 0, 0);
-            for (int k0 = 0; k0 < size; k0 += 8) {
-                float4 v[8];
-                float fk[8];
+            for (int c = 0; c < A.cluster; ++c) {
+                const float* p = pieces_of(c) + pr * d + i;
+                for (int k0 = 0; k0 < A.team; k0 += 4) {
+                    float4 v[4];
+                    float fk[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int kk = k0 + k;
-                    const bool there = kk < size && ((kk < 32 ? present[0] >> kk : present[1] >> (kk - 32)) & 1);
-                    fk[k] = there ? __shfl_sync(0xffffffffu, kk < 32 ? f[0] : f[1], kk & 31) : 0.0f;
-                    v[k] = there && i < d ? *reinterpret_cast<const float4*>(piece(kk) + (size_t)pr * d + i) : make_float4(0, 0, 0, 0);
+                    for (int k = 0; k < 4; ++k) {
+                        const int kk = c * A.team + k0 + k;
+                        const bool there = k0 + k < A.team && (((kk < 32 ? present[0] : present[1]) >> (kk & 31)) & 1);
+                        fk[k] = __shfl_sync(0xffffffffu, kk < 32 ? f[0] : f[1], kk & 31);
+                        if (!there) fk[k] = 0.0f;
+                        v[k] = there && i < d ? *reinterpret_cast<const float4*>(p + (k0 + k) * ring_floats) : make_float4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        a.x = fmaf(v[k].x, fk[k], a.x), a.y = fmaf(v[k].y, fk[k], a.y), a.z = fmaf(v[k].z, fk[k], a.z), a.w = fmaf(v[k].w, fk[k], a.w);
                 }
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    a.x = fmaf(v[k].x, fk[k], a.x), a.y = fmaf(v[k].y, fk[k], a.y), a.z = fmaf(v[k].z, fk[k], a.z), a.w = fmaf(v[k].w, fk[k], a.w);
             }
             if (i < d) *reinterpret_cast<float4*>(A.out + at * d + i) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
         }
