@@ -25,7 +25,8 @@
 //
 // Arithmetic. mma.sync m16n8k16 on f16 operands with f32 sums, at f32 accuracy: the operand with 16 rows holds eight heads
 // twice, rows 0-7 the leading f16 part of each f32 value and rows 8-15 the remainder (22 bits together), so query and
-// weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16. Query
+// weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16 (an
+// int8 key, raised by 128, as a subnormal: its bits are the integer, and the 128 leaves by what the sum begins with). Query
 // rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's
 // smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a value's scale s turns the two parts
 // (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'), whose bracket is exact in f16.
@@ -98,24 +99,42 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the same into fresh sums
-__device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+// the same into fresh sums: c in the first row half (heads' leading parts), 0 in the second
+__device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float first = 0.0f) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %11, %11};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(first), "f"(0.0f));
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+    float2 r;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
 __device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 // x, y as f16 leading parts and remainders
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = bits_of(h), lo = bits_of(__floats2half2_rn(x - f.x, y - f.y));
+    const float2 f = __half22float2(h), r = add2(make_float2(x, y), make_float2(-f.x, -f.y));
+    hi = bits_of(h), lo = bits_of(__floats2half2_rn(r.x, r.y));
 }
 // A sum over both halves of the 16-row operand. Where the leading part met an infinity the remainder's product is
 // meaningless (0 or a negative number times infinity).
@@ -128,6 +147,13 @@ __device__ __forceinline__ float whole(float lead, float rest) {
 template <int SEL>
 __device__ __forceinline__ uint32_t widen(uint32_t biased) {
     return bits_of(__hsub2(half2_of(__byte_perm(biased, 0x64646464u, SEL)), half2_of(0x64806480u)));
+}
+
+// The same as multiples of 2^-24: byte b + 128 as the bits of a subnormal f16, which the product takes exactly. The 128 is
+// taken out by what the sums begin with.
+template <int SEL>
+__device__ __forceinline__ uint32_t widen_low(uint32_t biased) {
+    return __byte_perm(biased, 0u, SEL);
 }
 
 // The keys sequence s sees; a length the call does not allow is cut and reported.
@@ -453,6 +479,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
 
     // ---- the share, piece by piece
     uint32_t qa[KS][4];
+    float q_bias[Q8 ? NB : 1];  // Q8_0: -128 times the sum of a block's query values, in the scores' unit of 2^-24
     float o[DM / 8][4], l_run = 0.0f, m_run = -INFINITY, m_use = 0.0f, row_scale = 1.0f;
     float v_cap = 0.0f, v_unit = 1.0f;  // Q8_0: value scales up to v_cap so far; sums count in multiples of v_unit (a power of two)
     __half2 v_norm = half2_of(0x3c003c00u);  // 1 / v_unit
@@ -506,6 +533,18 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                 split2(x[kk][0] * up * rest, x[kk][1] * up * rest, qa[kk][0], qa[kk][1]);
                 split2(x[kk][2] * up * rest, x[kk][3] * up * rest, qa[kk][2], qa[kk][3]);
             }
+            if (Q8) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += x[2 * b][i] + x[2 * b + 1][i];
+                    sum = sum * up * rest;
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    q_bias[b] = sum * (-128.0f / 16777216.0f);
+                }
+            }
             m_run = -INFINITY, m_use = 0.0f, l_run = 0.0f, v_cap = 0.0f, v_unit = 1.0f;
 #pragma unroll
             for (int n = 0; n < DM / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
@@ -519,7 +558,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         // ---- scores: keys 8 n + 2t, + 1 for head g
         cp_async_wait_oldest();
         ring_sync();  // the keys' copies of all the ring's warps have landed
-        float sc[NT][2];
+        float2 sc[NT];
         if (Q8) {
             const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage_at + k_scale_at);
 #pragma unroll
@@ -527,8 +566,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                 uint32_t w[4][(NB + 1) / 2];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) load_scales<NB, EXACT>(ksc + (n2 * 16 + 2 * t + (i & 1) + (i >> 1) * 8) * nb, nb, w[i]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[2 * n2 + (i >> 1)][i & 1] = 0.0f;
+                sc[2 * n2] = sc[2 * n2 + 1] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     if (EXACT || b < nb) {
@@ -537,17 +575,15 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                         float c0[4], c1[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
-                        mma16816_new(c0, qa[2 * b], widen<0x4140>(r[0]), widen<0x4342>(r[0]));
-                        mma16816_new(c1, qa[2 * b], widen<0x4140>(r[2]), widen<0x4342>(r[2]));
-                        mma16816(c0, qa[2 * b + 1], widen<0x4140>(r[1]), widen<0x4342>(r[1]));
-                        mma16816(c1, qa[2 * b + 1], widen<0x4140>(r[3]), widen<0x4342>(r[3]));
+                        mma16816_new(c0, qa[2 * b], widen_low<0x4140>(r[0]), widen_low<0x4342>(r[0]), q_bias[b]);
+                        mma16816_new(c1, qa[2 * b], widen_low<0x4140>(r[2]), widen_low<0x4342>(r[2]), q_bias[b]);
+                        mma16816(c0, qa[2 * b + 1], widen_low<0x4140>(r[1]), widen_low<0x4342>(r[1]));
+                        mma16816(c1, qa[2 * b + 1], widen_low<0x4140>(r[3]), widen_low<0x4342>(r[3]));
                         float f[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) f[i] = (b & 1) ? __high2float(half2_of(w[i][b / 2])) : __low2float(half2_of(w[i][b / 2]));
-                        sc[2 * n2][0] = fmaf(f[0], c0[0] + c0[2], sc[2 * n2][0]);
-                        sc[2 * n2][1] = fmaf(f[1], c0[1] + c0[3], sc[2 * n2][1]);
-                        sc[2 * n2 + 1][0] = fmaf(f[2], c1[0] + c1[2], sc[2 * n2 + 1][0]);
-                        sc[2 * n2 + 1][1] = fmaf(f[3], c1[1] + c1[3], sc[2 * n2 + 1][1]);
+                        sc[2 * n2] = fma2(make_float2(f[0], f[1]), add2(make_float2(c0[0], c0[1]), make_float2(c0[2], c0[3])), sc[2 * n2]);
+                        sc[2 * n2 + 1] = fma2(make_float2(f[2], f[3]), add2(make_float2(c1[0], c1[1]), make_float2(c1[2], c1[3])), sc[2 * n2 + 1]);
                     }
                 }
             }
@@ -571,7 +607,7 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) sc[n][0] = whole(c[n][0], c[n][2]), sc[n][1] = whole(c[n][1], c[n][3]);
+            for (int n = 0; n < NT; ++n) sc[n] = make_float2(whole(c[n][0], c[n][2]), whole(c[n][1], c[n][3]));
         }
         ring_sync();  // all the ring's warps are done with the keys
         if (left > 0) place(look);
@@ -581,12 +617,13 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         float top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            sc[n][0] *= row_scale, sc[n][1] *= row_scale;
+            if (Q8) sc[n] = mul2(sc[n], 16777216.0f);
+            sc[n] = mul2(sc[n], row_scale);
             if (partial) {
-                if (!takes_part(8 * n + 2 * t)) sc[n][0] = -INFINITY;
-                if (!takes_part(8 * n + 2 * t + 1)) sc[n][1] = -INFINITY;
+                if (!takes_part(8 * n + 2 * t)) sc[n].x = -INFINITY;
+                if (!takes_part(8 * n + 2 * t + 1)) sc[n].y = -INFINITY;
             }
-            top = fmaxf(top, fmaxf(sc[n][0], sc[n][1]));
+            top = fmaxf(top, fmaxf(sc[n].x, sc[n].y));
         }
         // the maximum moves rarely after the first units: the sums are touched only then
         if (__any_sync(0xffffffffu, top > m_run)) {
@@ -603,7 +640,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         uint32_t ph[NT], pl[NT];  // weights times 2^15 of two neighbouring keys, leading parts and remainders
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float p0 = ex2(fmaf(sc[n][0] - m_use, kLog2e, 15.0f)), p1 = ex2(fmaf(sc[n][1] - m_use, kLog2e, 15.0f));
+            const float2 e = fma2(add2(sc[n], make_float2(-m_use, -m_use)), make_float2(kLog2e, kLog2e), make_float2(15.0f, 15.0f));
+            const float p0 = ex2(e.x), p1 = ex2(e.y);
             l_run += p0 + p1;
             split2(p0, p1, ph[n], pl[n]);
         }
