@@ -26,7 +26,7 @@
 // Arithmetic. mma.sync m16n8k16 on f16 operands with f32 sums, at f32 accuracy: the operand with 16 rows holds eight heads
 // twice, rows 0-7 the leading f16 part of each f32 value and rows 8-15 the remainder (22 bits together), so query and
 // weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16 (an
-// int8 key, raised by 128, as a subnormal: its bits are the integer, and the 128 leaves by what the sum begins with). Query
+// int8 key, raised by 128, as a subnormal: its bits are the integer, and the sum begins with -128 times the query's). Query
 // rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's
 // smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a value's scale s turns the two parts
 // (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'), whose bracket is exact in f16.
@@ -99,7 +99,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the same into fresh sums: c in the first row half (heads' leading parts), 0 in the second
+// the same into fresh sums: `first` in the first row half (heads' leading parts), 0 in the second
 __device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float first = 0.0f) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %11, %11};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -149,8 +149,9 @@ __device__ __forceinline__ uint32_t widen(uint32_t biased) {
     return bits_of(__hsub2(half2_of(__byte_perm(biased, 0x64646464u, SEL)), half2_of(0x64806480u)));
 }
 
-// The same as multiples of 2^-24: byte b + 128 as the bits of a subnormal f16, which the product takes exactly. The 128 is
-// taken out by what the sums begin with.
+// The same as multiples of 2^-24: byte b + 128 as the bits of a subnormal f16, which the product takes exactly. The 128
+// times the query's sum is what the block's sum begins with, negative: the terms are some four times the true ones' size in
+// the root mean square, which costs two bits of 24 in a block's rounding.
 template <int SEL>
 __device__ __forceinline__ uint32_t widen_low(uint32_t biased) {
     return __byte_perm(biased, 0u, SEL);
@@ -1033,8 +1034,11 @@ struct Plan {
 // three where chunks are handed out.
 constexpr int kMinUnits = 2, kMinUnitsDynamic = 3;
 
-// Teams walk rows of at most this many units per ring: longer ones are better spread over all rings.
-constexpr int kTeamUnits = 8;
+// Teams walk rows of at most this many units per ring, longer ones are better spread over all rings: where the teams leave
+// SMs idle (one sequence of 4000 tokens, eight kv heads, f16: 19.5 us by teams of 24 rings, 5.3 units each, 15.5 us over all
+// rings; 8192 tokens 17.9 us over all rings, 22.1 us by teams of 48 rings in clusters of eight CTAs), and where they fill three
+// quarters of the GPU (16 sequences of 2000 tokens, Q8_0: 25.4 us by teams of 8 rings, 8 units each, 29.3 us over all rings).
+constexpr int kTeamUnits = 4, kTeamUnitsFull = 8;
 
 int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max_len, int sm_count, Plan* out) {
     Plan p;
@@ -1061,7 +1065,8 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     while (p.team > 1 && (rows + p.rings / p.team - 1) / (p.rings / p.team) > (size_t)sm_count) --p.team;
     while (p.cluster < 4 && p.team == p.rings && 2 * rows * p.cluster <= (size_t)sm_count && units > (size_t)p.team * p.cluster) p.cluster *= 2;
     // (a piece of a team lies on its ring's stages)
-    p.row_mode = units <= (size_t)kTeamUnits * p.team * p.cluster && (p.team * p.cluster == 1 || (size_t)2 * p.stage_bytes >= piece);
+    const bool full = 4 * ((rows + p.rings / p.team - 1) / (p.rings / p.team)) * p.cluster >= 3 * (size_t)sm_count;
+    p.row_mode = units <= (size_t)(full ? kTeamUnitsFull : kTeamUnits) * p.team * p.cluster && (p.team * p.cluster == 1 || (size_t)2 * p.stage_bytes >= piece);
     if (!p.row_mode) p.team = p.rings, p.cluster = 1;
     const size_t most = rows * units, rings_all = (size_t)sm_count * p.rings;
     p.dynamic = !p.row_mode && !q8 && most >= 48 * rings_all;
