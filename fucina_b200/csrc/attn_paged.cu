@@ -23,13 +23,17 @@
 // Copies. The keys of a stage are refilled as soon as the scores are taken, the values after the second product: nearly
 // two units per ring are in flight at any time from two stages' room.
 //
-// Arithmetic. mma.sync m16n8k16 on f16 operands with f32 sums, at f32 accuracy: the operand with 16 rows holds eight heads
-// twice, rows 0-7 the leading f16 part of each f32 value and rows 8-15 the remainder (22 bits together), so query and
-// weights are not rounded and the split costs no extra instruction; the cache's f16 or int8 values are exact in f16 (an
-// int8 key, raised by 128, as a subnormal: its bits are the integer, and the sum begins with -128 times the query's). Query
-// rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that remainders stay clear of f16's
-// smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a value's scale s turns the two parts
-// (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'), whose bracket is exact in f16.
+// Arithmetic. mma.sync m16n8k16 on f16 operands with f32 sums, at f32 accuracy: keys (then value columns) are the sixteen
+// rows of the first operand, and each query head is two neighbouring columns of the second, the leading f16 part of every
+// f32 value and the remainder (22 bits together), so query and weights are not rounded; the cache's f16 or int8 values are
+// exact in f16 (an int8 key, raised by 128, as a subnormal: its bits are the integer, and the sum begins with -128 times the
+// query's). Four heads fill the eight columns of an instruction (one tile of heads; a warp has one or two): with eight heads
+// as rows instead, groups of four heads, the usual ones, would leave half of every instruction and half of the softmax
+// empty. A lane holds one head of a tile throughout: its scores of keys g and g + 8, and its sums. Weights change from
+// sums to operands by movmatrix. Query rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that
+// remainders stay clear of f16's smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a
+// value's scale s turns the two parts (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'),
+// whose bracket is exact in f16.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -44,15 +48,15 @@ namespace {
 constexpr float kNegBig = -3.4e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSub = 16;       // keys that surely lie in one page
-constexpr int kRowsPerWarp = 8;
+constexpr int kTile = 4;       // query heads of a tile
 constexpr int kMaxRings = 16;  // 2 x kMaxRings pieces are joined by one lane each
 constexpr int kSmemMost = 226 * 1024;
 constexpr size_t kMaxLen = (size_t)1 << 28;
 
-// Keys per unit and warps per CTA for rows of up to `dm` values: what the registers (o is dm / 2 of them, the query as
-// many as a quarter of that again) and the stages' room allow.
+// Keys per unit and warps per CTA for rows of up to `dm` values and `tiles` tiles of heads a warp: what the registers (the
+// sums are tiles * dm / 4 of them, the query half as many) and the stages' room allow.
 __host__ __device__ constexpr int unit_keys(int dm) { return dm <= 128 ? 32 : 16; }
-__host__ __device__ constexpr int max_warps(int dm) { return dm <= 64 ? 12 : 8; }
+__host__ __device__ constexpr int max_warps(int dm, int tiles) { return dm * tiles <= 128 ? 12 : 8; }
 
 struct PagedArgs {
     KvView c;
@@ -68,7 +72,7 @@ struct PagedArgs {
     int* status;
     int passes;        // a kv head with more than 32 query heads is walked in this many rows of `span` heads
     int span;          // query heads of one row
-    int warps_per_ring, heads_per_warp, rings;
+    int warps_per_ring, heads_per_warp, rows_per_warp, rings;  // rows_per_warp: 4 or 8, heads_per_warp of them in use
     int stage_bytes;
     int row_mode;      // every row has a team of rings
     int team, cluster; // its rings in a CTA, and CTAs
@@ -79,7 +83,7 @@ struct PagedArgs {
     int* next;
     int* sums;         // [n_seqs + 1]
     int2* meta;        // per chunk: the row that begins in it and ends in a later one (-1: none), the chunk of the row's end
-    float* parts;      // per chunk [2][warps_per_ring * 8][d + 2] (o, then max and sum): a row that began earlier, a row that ends later
+    float* parts;      // per chunk [2][warps_per_ring * rows_per_warp][d + 2] (o, then max and sum): a row that began earlier, a row that ends later
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -99,11 +103,17 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// the same into fresh sums: `first` in the first row half (heads' leading parts), 0 in the second
+// the same into fresh sums: `first` in the even columns (heads' leading parts), 0 in the odd ones
 __device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float first = 0.0f) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %11, %11};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(first), "f"(0.0f));
+}
+// an 8 x 8 matrix of f16, a row's two neighbours per lane, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -136,7 +146,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     const float2 f = __half22float2(h), r = add2(make_float2(x, y), make_float2(-f.x, -f.y));
     hi = bits_of(h), lo = bits_of(__floats2half2_rn(r.x, r.y));
 }
-// A sum over both halves of the 16-row operand. Where the leading part met an infinity the remainder's product is
+// A sum over both columns of a head. Where the leading part met an infinity the remainder's product is
 // meaningless (0 or a negative number times infinity).
 __device__ __forceinline__ float whole(float lead, float rest) {
     const float x = lead + rest;
@@ -228,13 +238,13 @@ __device__ __forceinline__ void load_scales(const __half* row, int nb, uint32_t 
     }
 }
 
-// EXACT: rows have DM values; else up to DM
-template <bool Q8, int DM, bool EXACT>
-__global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const __grid_constant__ PagedArgs A) {
+// EXACT: rows have DM values; else up to DM. HT: tiles of four heads a warp
+template <bool Q8, int DM, bool EXACT, int HT>
+__global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(const __grid_constant__ PagedArgs A) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int sh_next[kMaxRings][2];
     pdl_wait_then_release();
-    constexpr int UK = unit_keys(DM), NT = UK / 8;  // keys of a unit, and groups of eight of them
+    constexpr int UK = unit_keys(DM);               // keys of a unit
     constexpr int KS = DM / 16, NB = DM / 32;       // 16-value steps and 32-value blocks of a row
     const bool dynamic = !Q8 && A.dynamic;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -244,7 +254,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     const int nc = Q8 ? d >> 4 : d >> 3;  // 16-byte chunks of a key's row
     const int pitch = (nc + 1) * 16;      // an odd number of chunks: the rows of an ldmatrix fall on distinct banks
     const int rows_per_seq = A.c.kv_heads * A.passes;
-    const int prow = A.warps_per_ring * kRowsPerWarp;  // head rows of a piece
+    constexpr int RPW = kTile * HT;
+    const int prow = A.warps_per_ring * RPW;  // head rows of a piece
     const int piece_floats = prow * (d + 2);
     // a stage: K rows, V rows, and for Q8_0 their scales [UK][d / 32]
     const int k_scale_at = 2 * UK * pitch, v_scale_at = k_scale_at + UK * 2 * nb;
@@ -479,76 +490,86 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
     }
 
     // ---- the share, piece by piece
-    uint32_t qa[KS][4];
-    float q_bias[Q8 ? NB : 1];  // Q8_0: -128 times the sum of a block's query values, in the scores' unit of 2^-24
-    float o[DM / 8][4], l_run = 0.0f, m_run = -INFINITY, m_use = 0.0f, row_scale = 1.0f;
+    uint32_t qb[HT][KS][2];
+    float q_bias[HT][Q8 ? NB : 1];  // Q8_0: -128 times the sum of a block's query values, in the scores' unit of 2^-24
+    float o[HT][DM / 16][4], l_run[HT], m_run[HT], m_use[HT], row_scale[HT];
     float v_cap = 0.0f, v_unit = 1.0f;  // Q8_0: value scales up to v_cap so far; sums count in multiples of v_unit (a power of two)
     __half2 v_norm = half2_of(0x3c003c00u);  // 1 / v_unit
     bool started = false, begun_here = false;
     uint32_t stage_at = 0;
     const int mi = lane >> 3, mr = lane & 7;
-    const uint32_t k_lane = (uint32_t)(((mi >> 1) * 8 + mr) * pitch + (mi & 1) * 16);
-    const uint32_t v_lane = (uint32_t)(((mi & 1) * 8 + mr) * pitch + (mi >> 1) * 16);
+    // addresses of a lane in an ldmatrix of four 8 x 8 matrices: (keys, keys + 8) then the next chunk, or the other way round
+    const uint32_t by_keys = (uint32_t)(((mi & 1) * 8 + mr) * pitch + (mi >> 1) * 16);
+    const uint32_t by_chunks = (uint32_t)(((mi >> 1) * 8 + mr) * pitch + (mi & 1) * 16);
 
     int done = 0;
     while (count > 0) {
         if (!started) {
             started = true;
             begun_here = cur.key == cur.first / UK * UK;
-            // query fragments: row g = head g of this warp, times a power of two that puts the row's largest value near 2^14
+            // query fragments: column g of tile h = head 4 h + g / 2 of this warp, leading parts (g even) or remainders, times a power
+            // of two that puts the row's largest value near 2^14. A lane's sums are those of head 4 h + t: what belongs to a head comes
+            // from lane 8 t.
             const int kvh = cur.r / A.passes, pass = cur.r - kvh * A.passes;
-            const int in_row = part * A.heads_per_warp + g, in_group = pass * A.span + in_row;
-            const bool live = g < A.heads_per_warp && in_row < A.span && in_group < A.group;
-            const float* qrow = A.q + (size_t)cur.s * A.q_stride + (size_t)(kvh * A.group + (live ? in_group : 0)) * d;
-            float x[KS][4];
-            float big = 0.0f;
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
+            for (int h = 0; h < HT; ++h) {
+                const int head = kTile * h + (g >> 1), in_row = part * A.heads_per_warp + head, in_group = pass * A.span + in_row;
+                const bool live = head < A.heads_per_warp && in_row < A.span && in_group < A.group;
+                const float* qrow = A.q + (size_t)cur.s * A.q_stride + (size_t)(kvh * A.group + (live ? in_group : 0)) * d;
+                float x[KS][4];
+                float big = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[kk][i] = 0.0f;
-                if (live && (EXACT || kk < steps)) {
-                    // f16: columns 2t, 2t + 1, 2t + 8, 2t + 9 of the step; Q8_0: 4t .. 4t + 3, the bytes a lane gets from ldmatrix
-                    if (Q8) {
-                        const float4 a = *reinterpret_cast<const float4*>(qrow + 16 * kk + 4 * t);
-                        x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = a.z, x[kk][3] = a.w;
-                    } else {
-                        const float2 a = *reinterpret_cast<const float2*>(qrow + 16 * kk + 2 * t), b = *reinterpret_cast<const float2*>(qrow + 16 * kk + 8 + 2 * t);
-                        x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = b.x, x[kk][3] = b.y;
+                for (int kk = 0; kk < KS; ++kk) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[kk][i] = 0.0f;
+                    if (live && (EXACT || kk < steps)) {
+                        // f16: columns 2t, 2t + 1, 2t + 8, 2t + 9 of the step; Q8_0: 4t .. 4t + 3, the bytes a lane gets from ldmatrix
+                        if (Q8) {
+                            const float4 a = *reinterpret_cast<const float4*>(qrow + 16 * kk + 4 * t);
+                            x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = a.z, x[kk][3] = a.w;
+                        } else {
+                            const float2 a = *reinterpret_cast<const float2*>(qrow + 16 * kk + 2 * t), b = *reinterpret_cast<const float2*>(qrow + 16 * kk + 8 + 2 * t);
+                            x[kk][0] = a.x, x[kk][1] = a.y, x[kk][2] = b.x, x[kk][3] = b.y;
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk)
+                for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[kk][i]));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // exponent e of big: rows are multiplied by 2^(14 - e), scores by scale * 2^(e - 14), each in two steps so that no
-            // factor overflows
-            const int e = big > 0.0f && big < INFINITY ? (int)((__float_as_uint(big) >> 23) & 255) - 126 : 0;
-            const int e1 = max(-120, min(120, 14 - e));
-            const float up = __int_as_float((127 + e1) << 23), rest = __int_as_float((127 + (14 - e) - e1) << 23);
-            row_scale = A.scale / up / rest;
+                    for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(x[kk][i]));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                // exponent e of big: rows are multiplied by 2^(14 - e), scores by scale * 2^(e - 14), each in two steps so that no
+                // factor overflows
+                const int e = big > 0.0f && big < INFINITY ? (int)((__float_as_uint(big) >> 23) & 255) - 126 : 0;
+                const int e1 = max(-120, min(120, 14 - e));
+                const float up = __int_as_float((127 + e1) << 23), rest = __int_as_float((127 + (14 - e) - e1) << 23);
+                row_scale[h] = __shfl_sync(0xffffffffu, A.scale / up / rest, 8 * t);
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                split2(x[kk][0] * up * rest, x[kk][1] * up * rest, qa[kk][0], qa[kk][1]);
-                split2(x[kk][2] * up * rest, x[kk][3] * up * rest, qa[kk][2], qa[kk][3]);
-            }
-            if (Q8) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sum += x[2 * b][i] + x[2 * b + 1][i];
-                    sum = sum * up * rest;
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    q_bias[b] = sum * (-128.0f / 16777216.0f);
+                for (int kk = 0; kk < KS; ++kk) {
+                    uint32_t hi, low;
+                    split2(x[kk][0] * up * rest, x[kk][1] * up * rest, hi, low);
+                    qb[h][kk][0] = g & 1 ? low : hi;
+                    split2(x[kk][2] * up * rest, x[kk][3] * up * rest, hi, low);
+                    qb[h][kk][1] = g & 1 ? low : hi;
                 }
-            }
-            m_run = -INFINITY, m_use = 0.0f, l_run = 0.0f, v_cap = 0.0f, v_unit = 1.0f;
+                if (Q8) {
 #pragma unroll
-            for (int n = 0; n < DM / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+                    for (int b = 0; b < NB; ++b) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sum += x[2 * b][i] + x[2 * b + 1][i];
+                        sum = sum * up * rest;
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                        q_bias[h][b] = __shfl_sync(0xffffffffu, sum * (-128.0f / 16777216.0f), 8 * t);
+                    }
+                }
+                m_run[h] = -INFINITY, m_use[h] = 0.0f, l_run[h] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < DM / 16; ++n) o[h][n][0] = o[h][n][1] = o[h][n][2] = o[h][n][3] = 0.0f;
+            }
+            v_cap = 0.0f, v_unit = 1.0f;
         }
         const int lo = max(cur.first - cur.key, 0), hi = min(cur.end - cur.key, UK);
         const unsigned lost = gone_now;
@@ -556,96 +577,110 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         const uint32_t ks = ring_addr + stage_at, vs = ks + UK * pitch;
         auto takes_part = [&](int key) { return key >= lo && key < hi && !((lost >> (key / kSub)) & 1); };
 
-        // ---- scores: keys 8 n + 2t, + 1 for head g
+        // ---- scores: keys 16 n + g (x) and 16 n + g + 8 (y) for head t of each tile
         cp_async_wait_oldest();
         ring_sync();  // the keys' copies of all the ring's warps have landed
-        float2 sc[NT];
+        float2 sc[HT][UK / 16];
         if (Q8) {
             const __half* ksc = reinterpret_cast<const __half*>(ring_base + stage_at + k_scale_at);
 #pragma unroll
-            for (int n2 = 0; n2 < NT / 2; ++n2) {  // sixteen keys at a time
-                uint32_t w[4][(NB + 1) / 2];
+            for (int n = 0; n < UK / 16; ++n) {
+                uint32_t w[2][(NB + 1) / 2];
+                load_scales<NB, EXACT>(ksc + (n * 16 + g) * nb, nb, w[0]);
+                load_scales<NB, EXACT>(ksc + (n * 16 + g + 8) * nb, nb, w[1]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) load_scales<NB, EXACT>(ksc + (n2 * 16 + 2 * t + (i & 1) + (i >> 1) * 8) * nb, nb, w[i]);
-                sc[2 * n2] = sc[2 * n2 + 1] = make_float2(0.0f, 0.0f);
+                for (int h = 0; h < HT; ++h) sc[h][n] = make_float2(0.0f, 0.0f);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     if (EXACT || b < nb) {
                         uint32_t r[4];
-                        ldsm_x4(ks + n2 * 16 * pitch + k_lane + b * 32, r);  // keys 0-7: values 0-15, 16-31 of the block; keys 8-15: the same
-                        float c0[4], c1[4];
+                        ldsm_x4(ks + n * 16 * pitch + by_keys + b * 32, r);  // values 0-15 of the block: keys 0-7, 8-15; values 16-31: the same
 #pragma unroll
                         for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
-                        mma16816_new(c0, qa[2 * b], widen_low<0x4140>(r[0]), widen_low<0x4342>(r[0]), q_bias[b]);
-                        mma16816_new(c1, qa[2 * b], widen_low<0x4140>(r[2]), widen_low<0x4342>(r[2]), q_bias[b]);
-                        mma16816(c0, qa[2 * b + 1], widen_low<0x4140>(r[1]), widen_low<0x4342>(r[1]));
-                        mma16816(c1, qa[2 * b + 1], widen_low<0x4140>(r[3]), widen_low<0x4342>(r[3]));
-                        float f[4];
+                        const uint32_t a0[4] = {widen_low<0x4140>(r[0]), widen_low<0x4140>(r[1]), widen_low<0x4342>(r[0]), widen_low<0x4342>(r[1])};
+                        const uint32_t a1[4] = {widen_low<0x4140>(r[2]), widen_low<0x4140>(r[3]), widen_low<0x4342>(r[2]), widen_low<0x4342>(r[3])};
+                        const float f0 = (b & 1) ? __high2float(half2_of(w[0][b / 2])) : __low2float(half2_of(w[0][b / 2]));
+                        const float f1 = (b & 1) ? __high2float(half2_of(w[1][b / 2])) : __low2float(half2_of(w[1][b / 2]));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) f[i] = (b & 1) ? __high2float(half2_of(w[i][b / 2])) : __low2float(half2_of(w[i][b / 2]));
-                        sc[2 * n2] = fma2(make_float2(f[0], f[1]), add2(make_float2(c0[0], c0[1]), make_float2(c0[2], c0[3])), sc[2 * n2]);
-                        sc[2 * n2 + 1] = fma2(make_float2(f[2], f[3]), add2(make_float2(c1[0], c1[1]), make_float2(c1[2], c1[3])), sc[2 * n2 + 1]);
+                        for (int h = 0; h < HT; ++h) {
+                            float c[4];
+                            mma16816_new(c, a0, qb[h][2 * b][0], qb[h][2 * b][1], q_bias[h][b]);
+                            mma16816(c, a1, qb[h][2 * b + 1][0], qb[h][2 * b + 1][1]);
+                            sc[h][n].x = fmaf(f0, c[0] + c[1], sc[h][n].x);
+                            sc[h][n].y = fmaf(f1, c[2] + c[3], sc[h][n].y);
+                        }
                     }
                 }
             }
         } else {
-            float c[NT][4];
+            float c[HT][UK / 16][4];
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
                 if (EXACT || kk < steps) {
 #pragma unroll
-                    for (int n2 = 0; n2 < NT / 2; ++n2) {
+                    for (int n = 0; n < UK / 16; ++n) {
                         uint32_t r[4];
-                        ldsm_x4(ks + n2 * 16 * pitch + k_lane + kk * 32, r);  // keys 0-7: values 0-7, 8-15 of the step; keys 8-15: the same
-                        if (kk == 0) {
-                            mma16816_new(c[2 * n2], qa[kk], r[0], r[1]);
-                            mma16816_new(c[2 * n2 + 1], qa[kk], r[2], r[3]);
-                        } else {
-                            mma16816(c[2 * n2], qa[kk], r[0], r[1]);
-                            mma16816(c[2 * n2 + 1], qa[kk], r[2], r[3]);
+                        ldsm_x4(ks + n * 16 * pitch + by_keys + kk * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
+#pragma unroll
+                        for (int h = 0; h < HT; ++h) {
+                            if (kk == 0) mma16816_new(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
+                            else mma16816(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
                         }
                     }
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) sc[n] = make_float2(whole(c[n][0], c[n][2]), whole(c[n][1], c[n][3]));
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int n = 0; n < UK / 16; ++n) sc[h][n] = make_float2(whole(c[h][n][0], c[h][n][1]), whole(c[h][n][2], c[h][n][3]));
         }
         ring_sync();  // all the ring's warps are done with the keys
         if (left > 0) place(look);
         copy_side(stage_at, 0);
 
         // ---- weights
-        float top = -INFINITY;
+        float top[HT];
+        bool moved = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (Q8) sc[n] = mul2(sc[n], 16777216.0f);
-            sc[n] = mul2(sc[n], row_scale);
-            if (partial) {
-                if (!takes_part(8 * n + 2 * t)) sc[n].x = -INFINITY;
-                if (!takes_part(8 * n + 2 * t + 1)) sc[n].y = -INFINITY;
+        for (int h = 0; h < HT; ++h) {
+            top[h] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < UK / 16; ++n) {
+                if (Q8) sc[h][n] = mul2(sc[h][n], 16777216.0f);
+                sc[h][n] = mul2(sc[h][n], row_scale[h]);
+                if (partial) {
+                    if (!takes_part(16 * n + g)) sc[h][n].x = -INFINITY;
+                    if (!takes_part(16 * n + g + 8)) sc[h][n].y = -INFINITY;
+                }
+                top[h] = fmaxf(top[h], fmaxf(sc[h][n].x, sc[h][n].y));
             }
-            top = fmaxf(top, fmaxf(sc[n].x, sc[n].y));
+            moved = moved || top[h] > m_run[h];
         }
         // the maximum moves rarely after the first units: the sums are touched only then
-        if (__any_sync(0xffffffffu, top > m_run)) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m_new = fmaxf(m_run, top);
-            const float r = m_run == -INFINITY ? 0.0f : ex2((m_run - m_new) * kLog2e);
-            m_run = m_new;
-            m_use = m_new == -INFINITY ? 0.0f : m_new;
-            l_run *= r;
+        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int n = 0; n < DM / 8; ++n) o[n][0] *= r, o[n][1] *= r, o[n][2] *= r, o[n][3] *= r;
-        }
-        uint32_t ph[NT], pl[NT];  // weights times 2^15 of two neighbouring keys, leading parts and remainders
+            for (int h = 0; h < HT; ++h) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float2 e = fma2(add2(sc[n], make_float2(-m_use, -m_use)), make_float2(kLog2e, kLog2e), make_float2(15.0f, 15.0f));
-            const float p0 = ex2(e.x), p1 = ex2(e.y);
-            l_run += p0 + p1;
-            split2(p0, p1, ph[n], pl[n]);
+                for (int x = 4; x <= 16; x <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
+                const float m_new = fmaxf(m_run[h], top[h]);
+                const float r = m_run[h] == -INFINITY ? 0.0f : ex2((m_run[h] - m_new) * kLog2e);
+                m_run[h] = m_new;
+                m_use[h] = m_new == -INFINITY ? 0.0f : m_new;
+                l_run[h] *= r;
+#pragma unroll
+                for (int n = 0; n < DM / 16; ++n) o[h][n][0] *= r, o[h][n][1] *= r, o[h][n][2] *= r, o[h][n][3] *= r;
+            }
         }
+        uint32_t ph[HT][UK / 16], pl[HT][UK / 16];  // weights times 2^15 of keys g and g + 8, leading parts and remainders
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int n = 0; n < UK / 16; ++n) {
+                const float2 e = fma2(add2(sc[h][n], make_float2(-m_use[h], -m_use[h])), make_float2(kLog2e, kLog2e), make_float2(15.0f, 15.0f));
+                const float p0 = ex2(e.x), p1 = ex2(e.y);
+                l_run[h] += p0 + p1;
+                split2(p0, p1, ph[h][n], pl[h][n]);
+            }
 
         // ---- values
         cp_async_wait_oldest();
@@ -665,20 +700,20 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         }
         if (Q8) {
             const __half* vsc = reinterpret_cast<const __half*>(ring_base + stage_at + v_scale_at);
-            uint32_t w[2 * NT][(NB + 1) / 2];
+            uint32_t w[UK / 8][(NB + 1) / 2];
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) load_scales<NB, EXACT>(vsc + (8 * (i >> 1) + 2 * t + (i & 1)) * nb, nb, w[i]);
+            for (int i = 0; i < UK / 8; ++i) load_scales<NB, EXACT>(vsc + (8 * i + g) * nb, nb, w[i]);
             // 2^15 times a scale above 1 may pass f16's range, and products with scales below 2^-9 lose their remainders to f16's
             // smallest steps: then the scales are taken relative to a power of two at or above the largest so far
             __half2 most2 = half2_of(w[0][0]);
 #pragma unroll
-            for (int i = 0; i < 2 * NT; ++i)
+            for (int i = 0; i < UK / 8; ++i)
 #pragma unroll
                 for (int b = 0; b < (NB + 1) / 2; ++b) most2 = __hmax2(most2, half2_of(w[i][b]));
             float most = fmaxf(__low2float(most2), __high2float(most2));
             if (__any_sync(0xffffffffu, most > v_cap)) {
 #pragma unroll
-                for (int x = 1; x <= 2; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                for (int x = 4; x <= 16; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
                 float unit = 1.0f;
                 v_cap = 1.0f;
                 if (most > 1.0f || most <= 1.0f / 512) {
@@ -690,47 +725,50 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
                 v_norm = __float2half2_rn(1.0f / unit);
                 // an earlier unit's sums count in the old unit; the cap never falls
 #pragma unroll
-                for (int n = 0; n < DM / 8; ++n) o[n][0] *= r, o[n][1] *= r, o[n][2] *= r, o[n][3] *= r;
+                for (int h = 0; h < HT; ++h)
+#pragma unroll
+                    for (int n = 0; n < DM / 16; ++n) o[h][n][0] *= r, o[h][n][1] *= r, o[h][n][2] *= r, o[h][n][3] *= r;
             }
             const bool plain = v_unit == 1.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (EXACT || b < nb) {
-                    uint32_t a[NT][2];  // leading parts and remainders of weight times scale
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
+                    for (int n = 0; n < UK / 16; ++n) {
                         __half2 s2 = half2_of(__byte_perm(w[2 * n][b / 2], w[2 * n + 1][b / 2], (b & 1) ? 0x7632 : 0x5410));
                         if (!plain) s2 = __hmul2(s2, v_norm);
-                        const __half2 hi2 = __hmul2(half2_of(ph[n]), s2);
-                        const __half2 rest = __hfma2(half2_of(ph[n]), s2, __hneg2(hi2));
-                        a[n][0] = bits_of(hi2), a[n][1] = bits_of(__hfma2(half2_of(pl[n]), s2, rest));
-                    }
-#pragma unroll
-                    for (int n2 = 0; n2 < NT / 2; ++n2) {
                         uint32_t r[4];
-                        const uint32_t aa[4] = {a[2 * n2][0], a[2 * n2][1], a[2 * n2 + 1][0], a[2 * n2 + 1][1]};
-                        ldsm_x4_t(vs + n2 * 16 * pitch + v_lane + b * 32, r);  // values 0-15 of the block: keys 0-7, 8-15; values 16-31: the same
+                        ldsm_x4_t(vs + n * 16 * pitch + by_keys + b * 32, r);  // values 0-15 of the block: keys 0-7, 8-15; values 16-31: the same
 #pragma unroll
                         for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
-                        // a lane's word: values 2g, 2g + 1 of key 2t, then of key 2t + 1
-                        mma16816(o[4 * b], aa, widen<0x4240>(r[0]), widen<0x4240>(r[1]));
-                        mma16816(o[4 * b + 1], aa, widen<0x4341>(r[0]), widen<0x4341>(r[1]));
-                        mma16816(o[4 * b + 2], aa, widen<0x4240>(r[2]), widen<0x4240>(r[3]));
-                        mma16816(o[4 * b + 3], aa, widen<0x4341>(r[2]), widen<0x4341>(r[3]));
+                        // a lane's word: values 2g, 2g + 1 of key 2t, then of key 2t + 1: rows g are the even values, rows g + 8 the odd ones
+                        const uint32_t a0[4] = {widen<0x4240>(r[0]), widen<0x4341>(r[0]), widen<0x4240>(r[1]), widen<0x4341>(r[1])};
+                        const uint32_t a1[4] = {widen<0x4240>(r[2]), widen<0x4341>(r[2]), widen<0x4240>(r[3]), widen<0x4341>(r[3])};
+#pragma unroll
+                        for (int h = 0; h < HT; ++h) {
+                            const __half2 lead = __hmul2(half2_of(ph[h][n]), s2);
+                            const __half2 rest = __hfma2(half2_of(pl[h][n]), s2, __hfma2(half2_of(ph[h][n]), s2, __hneg2(lead)));
+                            const uint32_t b0 = transposed(__byte_perm(bits_of(lead), bits_of(rest), 0x5410)), b1 = transposed(__byte_perm(bits_of(lead), bits_of(rest), 0x7632));
+                            mma16816(o[h][2 * b], a0, b0, b1);
+                            mma16816(o[h][2 * b + 1], a1, b0, b1);
+                        }
                     }
                 }
             }
         } else {
 #pragma unroll
-            for (int n2 = 0; n2 < NT / 2; ++n2) {
-                const uint32_t a[4] = {ph[2 * n2], pl[2 * n2], ph[2 * n2 + 1], pl[2 * n2 + 1]};
+            for (int n = 0; n < UK / 16; ++n) {
+                uint32_t b0[HT], b1[HT];
 #pragma unroll
-                for (int n = 0; n < KS; ++n) {
-                    if (EXACT || n < steps) {
+                for (int h = 0; h < HT; ++h)
+                    b0[h] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x5410)), b1[h] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x7632));
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    if (EXACT || k < steps) {
                         uint32_t r[4];
-                        ldsm_x4_t(vs + n2 * 16 * pitch + v_lane + n * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
-                        mma16816(o[2 * n], a, r[0], r[1]);
-                        mma16816(o[2 * n + 1], a, r[2], r[3]);
+                        ldsm_x4_t(vs + n * 16 * pitch + by_chunks + k * 32, r);  // keys 0-7: values 0-7, 8-15 of the step; keys 8-15: the same
+#pragma unroll
+                        for (int h = 0; h < HT; ++h) mma16816(o[h][k], r, b0[h], b1[h]);
                     }
                 }
             }
@@ -742,40 +780,40 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
 
         const bool ended = cur.left == 1, chunk_over = ++done == count;
         if (ended || chunk_over) {
-            l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-            l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-            const int in_row = part * A.heads_per_warp + g, kvh = cur.r / A.passes, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
+            const int kvh = cur.r / A.passes;
             const bool finished = begun_here && ended;
-            const bool live = g < A.heads_per_warp && in_row < A.span && in_group < A.group;
             const int which = begun_here ? 1 : 0;
-            const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
             if (A.row_mode && !finished) ring_sync();  // the piece lands on the ring's stages: all its warps are done with them
             float* pc = A.row_mode ? reinterpret_cast<float*>(ring_base) : A.parts + ((size_t)chunk * 2 + which) * piece_floats;
-            float* dst = finished ? A.out + at * d : pc + (size_t)(part * kRowsPerWarp + g) * d;
-            const float f = finished ? (l_run > 0.0f || l_run != l_run ? v_unit / l_run : 0.0f) : v_unit;
-            if (live || !finished) {
 #pragma unroll
-                for (int n = 0; n < KS; ++n) {
-                    if (EXACT || n < steps) {
-                        const float a = whole(o[2 * n][0], o[2 * n][2]) * f, b = whole(o[2 * n][1], o[2 * n][3]) * f;
-                        const float c = whole(o[2 * n + 1][0], o[2 * n + 1][2]) * f, e = whole(o[2 * n + 1][1], o[2 * n + 1][3]) * f;
-                        if (Q8) {
-                            *reinterpret_cast<float4*>(dst + 16 * n + 4 * t) = make_float4(a, c, b, e);
-                        } else {
-                            *reinterpret_cast<float2*>(dst + 16 * n + 2 * t) = make_float2(a, b);
-                            *reinterpret_cast<float2*>(dst + 16 * n + 8 + 2 * t) = make_float2(c, e);
+            for (int h = 0; h < HT; ++h) {
+                float l = l_run[h];
+#pragma unroll
+                for (int x = 4; x <= 16; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+                const int head = kTile * h + t, in_row = part * A.heads_per_warp + head, in_group = (cur.r - kvh * A.passes) * A.span + in_row;
+                const bool live = head < A.heads_per_warp && in_row < A.span && in_group < A.group;
+                const size_t at = (size_t)cur.s * A.heads + (size_t)kvh * A.group + in_group;
+                float* dst = finished ? A.out + at * d : pc + (size_t)(part * RPW + head) * d;
+                const float f = finished ? (l > 0.0f || l != l ? v_unit / l : 0.0f) : v_unit;
+                if (live || !finished) {
+#pragma unroll
+                    for (int n = 0; n < KS; ++n) {
+                        if (EXACT || n < steps) {
+                            const float a = whole(o[h][n][0], o[h][n][1]) * f, b = whole(o[h][n][2], o[h][n][3]) * f;
+                            if (Q8) *reinterpret_cast<float2*>(dst + 16 * n + 2 * g) = make_float2(a, b);
+                            else dst[16 * n + g] = a, dst[16 * n + g + 8] = b;
                         }
                     }
                 }
+                if (finished) {
+                    if (A.stats && live && g == 0) A.stats[at * 2] = l > 0.0f ? m_run[h] : kNegBig, A.stats[at * 2 + 1] = l * (1.0f / 32768.0f);
+                } else if (g == 0) {
+                    float* ml = pc + (size_t)prow * d + (part * RPW + head) * 2;
+                    ml[0] = m_run[h], ml[1] = l;
+                }
             }
-            if (finished) {
-                if (A.stats && live && t == 0) A.stats[at * 2] = l_run > 0.0f ? m_run : kNegBig, A.stats[at * 2 + 1] = l_run * (1.0f / 32768.0f);
-            } else {
-                float* ml = pc + (size_t)prow * d + (part * kRowsPerWarp + g) * 2;
-                if (t == 0) ml[0] = m_run, ml[1] = l_run;
-                if (which == 1 && !A.row_mode && part == 0 && lane == 0)
-                    A.meta[chunk] = make_int2(cur.s * rows_per_seq + cur.r, split.chunk_of(split.begin(chunk) + done - 1 + cur.left - 1));
-            }
+            if (!finished && which == 1 && !A.row_mode && part == 0 && lane == 0)
+                A.meta[chunk] = make_int2(cur.s * rows_per_seq + cur.r, split.chunk_of(split.begin(chunk) + done - 1 + cur.left - 1));
             if (chunk_over && !A.row_mode && (finished || which == 0) && part == 0 && lane == 0) A.meta[chunk] = make_int2(-1, -1);
             started = false;
         }
@@ -799,8 +837,8 @@ __global__ void __launch_bounds__(max_warps(DM) * 32, 1) attn_paged_kernel(const
         const int in_cta = item / prow, pr = item - in_cta * prow, row = blockIdx.x / A.cluster * teams + in_cta;
         if (row >= A.n_seqs * rows_per_seq) continue;
         const int s = row / rows_per_seq, r = row - s * rows_per_seq, kvh = r / A.passes;
-        const int in_row = (pr >> 3) * A.heads_per_warp + (pr & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
-        if ((pr & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) continue;
+        const int in_row = pr / RPW * A.heads_per_warp + pr % RPW, in_group = (r - kvh * A.passes) * A.span + in_row;
+        if (pr % RPW >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) continue;
         const int units = sh_next[in_cta * A.team][0];
         if (units == 1) continue;  // finished by its ring
         // ring k of the team's part in CTA c
@@ -911,7 +949,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
     __shared__ int sh_count[2];
     pdl_wait_then_release();
     const int d = A.c.d, w = threadIdx.x >> 5, lane = threadIdx.x & 31, threads = kJoinWarps * 32;
-    const int prow = A.warps_per_ring * kRowsPerWarp, rows_per_seq = A.c.kv_heads * A.passes;
+    const int prow = A.warps_per_ring * A.rows_per_warp, rows_per_seq = A.c.kv_heads * A.passes;
     const size_t piece_floats = (size_t)prow * (d + 2);
     int chunks = rings;
     if (A.dynamic) {
@@ -959,8 +997,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
     // where item `it` goes: the head's place in out, or -1
     auto place_of = [&](const int4& it) {
         const int s = it.z / rows_per_seq, r = it.z - s * rows_per_seq, kvh = r / A.passes;
-        const int in_row = (it.y >> 3) * A.heads_per_warp + (it.y & 7), in_group = (r - kvh * A.passes) * A.span + in_row;
-        if ((it.y & 7) >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) return -1ll;
+        const int in_row = it.y / A.rows_per_warp * A.heads_per_warp + it.y % A.rows_per_warp, in_group = (r - kvh * A.passes) * A.span + in_row;
+        if (it.y % A.rows_per_warp >= A.heads_per_warp || in_row >= A.span || in_group >= A.group) return -1ll;
         return (long long)s * A.heads + (long long)kvh * A.group + in_group;
     };
     const long long items = (long long)chunks * prow;
@@ -1025,7 +1063,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 
 // How a call is cut, from sizes the host knows.
 struct Plan {
-    int dm, exact, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
+    int dm, exact, tiles, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
     int row_mode, team, cluster, dynamic, grid, chunks;
     size_t smem, sums_at, meta_at, parts_at, workspace;
 };
@@ -1047,13 +1085,15 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     p.dm = d <= 64 && p.exact ? 64 : d <= 128 ? 128 : 256;
     p.passes = (group + 31) / 32;
     p.span = (group + p.passes - 1) / p.passes;
-    p.warps_per_ring = (p.span + kRowsPerWarp - 1) / kRowsPerWarp;
+    p.tiles = p.span <= kTile ? 1 : 2;
+    const int rows_per_warp = kTile * p.tiles;
+    p.warps_per_ring = (p.span + rows_per_warp - 1) / rows_per_warp;
     p.heads_per_warp = (p.span + p.warps_per_ring - 1) / p.warps_per_ring;
     const int keys = unit_keys(p.dm), pitch = ((q8 ? d / 16 : d / 8) + 1) * 16;
     p.stage_bytes = 2 * keys * pitch + (q8 ? 4 * keys * (d / 32) : 0);
-    const size_t piece = (size_t)p.warps_per_ring * kRowsPerWarp * (d + 2) * sizeof(float);
+    const size_t piece = (size_t)p.warps_per_ring * rows_per_warp * (d + 2) * sizeof(float);
     // as many rings as warps and two stages each allow
-    p.rings = max_warps(p.dm) / p.warps_per_ring;
+    p.rings = max_warps(p.dm, p.tiles) / p.warps_per_ring;
     while (p.rings > 1 && p.rings * 2 * p.stage_bytes > kSmemMost) --p.rings;
     if (p.rings * 2 * p.stage_bytes > kSmemMost) return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
     p.smem = (size_t)p.rings * 2 * p.stage_bytes;
@@ -1084,16 +1124,16 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     return FQ_OK;
 }
 
-template <bool Q8, int DM, bool EXACT>
+template <bool Q8, int DM, bool EXACT, int HT>
 cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
     static bool granted = false;  // under the dispatch lock
     if (!granted) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<Q8, DM, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<Q8, DM, EXACT, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
         if (e != cudaSuccess) return e;
         granted = true;
     }
     const dim3 grid((unsigned)p.grid), block((unsigned)(p.rings * p.warps_per_ring * 32));
-    if (p.cluster == 1) return launch_pdl(attn_paged_kernel<Q8, DM, EXACT>, grid, block, p.smem, st, a);
+    if (p.cluster == 1) return launch_pdl(attn_paged_kernel<Q8, DM, EXACT, HT>, grid, block, p.smem, st, a);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = p.smem, cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -1102,13 +1142,13 @@ cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr, cfg.numAttrs = getenv("FUCINA_B200_NO_PDL") ? 1 : 2;
-    return cudaLaunchKernelEx(&cfg, attn_paged_kernel<Q8, DM, EXACT>, a);
+    return cudaLaunchKernelEx(&cfg, attn_paged_kernel<Q8, DM, EXACT, HT>, a);
 }
-template <bool Q8>
+template <bool Q8, int HT>
 cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
-    if (p.dm == 64) return launch_paged<Q8, 64, true>(a, p, st);
-    if (p.dm == 128) return p.exact ? launch_paged<Q8, 128, true>(a, p, st) : launch_paged<Q8, 128, false>(a, p, st);
-    return p.exact ? launch_paged<Q8, 256, true>(a, p, st) : launch_paged<Q8, 256, false>(a, p, st);
+    if (p.dm == 64) return launch_paged<Q8, 64, true, HT>(a, p, st);
+    if (p.dm == 128) return p.exact ? launch_paged<Q8, 128, true, HT>(a, p, st) : launch_paged<Q8, 128, false, HT>(a, p, st);
+    return p.exact ? launch_paged<Q8, 256, true, HT>(a, p, st) : launch_paged<Q8, 256, false, HT>(a, p, st);
 }
 
 int check_paged(const fq_kv_pages* pages, size_t n_seqs, size_t heads, KvView* c) {
@@ -1180,7 +1220,7 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.q = q_dev, a.q_stride = q_stride, a.table = page_table_dev, a.len = kv_len_dev;
     a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages, a.max_len = (int)max_len, a.heads = (int)heads, a.group = (int)heads / c.kv_heads;
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
-    a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp;
+    a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp, a.rows_per_warp = kTile * p.tiles;
     a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.team = p.team, a.cluster = p.cluster, a.dynamic = p.dynamic;
     a.min_units = p.dynamic ? kMinUnitsDynamic : kMinUnits;
     const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
@@ -1192,10 +1232,10 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
         e = launch_pdl(unit_keys(p.dm) == 32 ? attn_paged_plan_kernel<32> : attn_paged_plan_kernel<16>, dim3(1), dim3(1024), 0, st, a);
         g_trace.launches++;
     }
-    if (e == cudaSuccess) e = q8 ? launch_paged<true>(a, p, st) : launch_paged<false>(a, p, st);
+    if (e == cudaSuccess) e = p.tiles == 1 ? (q8 ? launch_paged<true, 1>(a, p, st) : launch_paged<false, 1>(a, p, st)) : q8 ? launch_paged<true, 2>(a, p, st) : launch_paged<false, 2>(a, p, st);
     g_trace.launches++;
     if (e == cudaSuccess && !p.row_mode) {
-        const size_t items = (size_t)p.chunks * p.warps_per_ring * kRowsPerWarp, blocks = (size_t)ctx->sm_count * 4;
+        const size_t items = (size_t)p.chunks * p.warps_per_ring * a.rows_per_warp, blocks = (size_t)ctx->sm_count * 4;
         e = launch_pdl(attn_paged_join_kernel, dim3((unsigned)(items < blocks ? items : blocks)), dim3(kJoinWarps * 32), 0, st, a, p.grid * p.rings);
         g_trace.launches++;
     }
