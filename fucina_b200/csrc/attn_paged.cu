@@ -138,6 +138,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
+// The products of a unit join the running sums by f32 additions: the tensor instruction drops the bits of its sum that do not
+// fit, and over a chunk of some hundred instructions those losses, all towards zero, add up (64 f16 sequences of up to 8000
+// tokens: 1.7e-6 from the 64-bit result with the running sums inside the instruction, 0.7e-6 apart).
+__device__ __forceinline__ void add_to(float (&o)[4], const float (&c)[4]) {
+    const float2 a = add2(make_float2(o[0], o[1]), make_float2(c[0], c[1])), b = add2(make_float2(o[2], o[3]), make_float2(c[2], c[3]));
+    o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
+}
 __device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 half2_of(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 // x, y as f16 leading parts and remainders
@@ -733,6 +740,7 @@ __global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(c
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (EXACT || b < nb) {
+                    float c0[HT][4], c1[HT][4];
 #pragma unroll
                     for (int n = 0; n < UK / 16; ++n) {
                         __half2 s2 = half2_of(__byte_perm(w[2 * n][b / 2], w[2 * n + 1][b / 2], (b & 1) ? 0x7632 : 0x5410));
@@ -749,27 +757,37 @@ __global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(c
                             const __half2 lead = __hmul2(half2_of(ph[h][n]), s2);
                             const __half2 rest = __hfma2(half2_of(pl[h][n]), s2, __hfma2(half2_of(ph[h][n]), s2, __hneg2(lead)));
                             const uint32_t b0 = transposed(__byte_perm(bits_of(lead), bits_of(rest), 0x5410)), b1 = transposed(__byte_perm(bits_of(lead), bits_of(rest), 0x7632));
-                            mma16816(o[h][2 * b], a0, b0, b1);
-                            mma16816(o[h][2 * b + 1], a1, b0, b1);
+                            if (n == 0) mma16816_new(c0[h], a0, b0, b1), mma16816_new(c1[h], a1, b0, b1);
+                            else mma16816(c0[h], a0, b0, b1), mma16816(c1[h], a1, b0, b1);
                         }
                     }
+#pragma unroll
+                    for (int h = 0; h < HT; ++h) add_to(o[h][2 * b], c0[h]), add_to(o[h][2 * b + 1], c1[h]);
                 }
             }
         } else {
+            uint32_t b0[HT][UK / 16], b1[HT][UK / 16];
 #pragma unroll
-            for (int n = 0; n < UK / 16; ++n) {
-                uint32_t b0[HT], b1[HT];
+            for (int h = 0; h < HT; ++h)
 #pragma unroll
-                for (int h = 0; h < HT; ++h)
-                    b0[h] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x5410)), b1[h] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x7632));
+                for (int n = 0; n < UK / 16; ++n)
+                    b0[h][n] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x5410)), b1[h][n] = transposed(__byte_perm(ph[h][n], pl[h][n], 0x7632));
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    if (EXACT || k < steps) {
+            for (int k = 0; k < KS; ++k) {
+                if (EXACT || k < steps) {
+                    float c[HT][4];
+#pragma unroll
+                    for (int n = 0; n < UK / 16; ++n) {
                         uint32_t r[4];
                         ldsm_x4_t(vs + n * 16 * pitch + by_chunks + k * 32, r);  // keys 0-7: values 0-7, 8-15 of the step; keys 8-15: the same
 #pragma unroll
-                        for (int h = 0; h < HT; ++h) mma16816(o[h][k], r, b0[h], b1[h]);
+                        for (int h = 0; h < HT; ++h) {
+                            if (n == 0) mma16816_new(c[h], r, b0[h][n], b1[h][n]);
+                            else mma16816(c[h], r, b0[h][n], b1[h][n]);
+                        }
                     }
+#pragma unroll
+                    for (int h = 0; h < HT; ++h) add_to(o[h][k], c[h]);
                 }
             }
         }

@@ -210,7 +210,8 @@ FQ_API int fq_kv_read_dev(const fq_kv_pages* pages, void* k_out_dev, void* v_out
  * FQ_ERR_PAGE. It sizes the workspace and picks the split, so a replayed graph serves every length up to it.
  * workspace_dev: fq_attn_paged_workspace_bytes of device memory, 16-byte aligned, contents irrelevant before and after;
  * one call at a time may use it (two graphs that may run at the same time need one each). NULL: taken from the
- * library's caching allocator for the call (declined while the stream is being captured). Same inputs give the same
+ * library's caching allocator for the call (declined while the stream is being captured). Its size follows from max_len (as
+ * in the call; max_pages * page_tokens where the call says 0), is 0 for short max_len and needs fq_init. Same inputs give the same
  * bits whatever else runs. heads <= 4096, n_seqs <= 65535, max_len <= 2^28. */
 FQ_API size_t fq_attn_paged_workspace_bytes(const fq_kv_pages* pages, size_t n_seqs, size_t heads, size_t max_len);
 FQ_API int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_stride, const int32_t* page_table_dev,

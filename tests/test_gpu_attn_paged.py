@@ -38,6 +38,7 @@ def run(P, kind, lens, page, heads, kv, d, window=0, seed=1, gain=1.0, max_len=0
     ([200, 90], 16, 9, 1, 32, 0),
     ([300, 40], 16, 80, 1, 64, 0),                  # eighty heads to a kv head
     ([260], 256, 6, 3, 160, 0),
+    ([5000, 20], 4096, 4, 1, 64, 0),                # pages longer than most sequences
     ([180, 5], 16, 17, 1, 160, 0),                  # seventeen heads of 160
     ([300, 290], 16, 31, 1, 192, 0),
     ([120, 300], 32, 4, 2, 256, 0),
@@ -306,6 +307,80 @@ def test_captured_steps_follow_the_lengths(P):
             check_attention(w["cache"], rows, w["qh"], w["out"].cpu().numpy(), float(np.float32(0.09)))
     for w in worlds:
         w["graph"].destroy()
+
+
+def test_a_captured_call_needs_a_workspace_of_its_own(P):
+    import torch
+
+    rng = np.random.default_rng(25)
+    cache = Cache(P, "f16", [9000], 64, 1, 128, rng)
+    q, out = torch.zeros(1, 4, 128).cuda(), torch.zeros(1, 4, 128).cuda()
+    size = P.attn_paged_workspace_bytes(cache.pages, 1, 4, 9000)
+    assert size > 0
+    ws = torch.empty(size, dtype=torch.uint8).cuda()
+    torch.cuda.synchronize()
+    args = (cache.pages, q, out, cache.table, cache.lens_dev, 1, cache.max_pages, 4, 0.1)
+    with P.capture() as cap:
+        with pytest.raises(P.Declined):
+            P.attn_paged_dev(*args)
+        with pytest.raises(P.Declined):
+            P.attn_paged_dev(*args, workspace=ws, workspace_bytes=size - 16)
+        P.attn_paged_dev(*args, workspace=ws, workspace_bytes=size)
+    cap.graph.launch()
+    P.synchronize()
+    cap.graph.destroy()
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+def test_two_streams_at_once(P, kind):
+    """Calls on two streams without an order between them, each with its own workspace or the library's."""
+    import torch
+
+    rng = np.random.default_rng(26)
+    cache = Cache(P, kind, [6000, 40, 3000], 16, 2, 128, rng)
+    cache.fill(rng)
+    q = rng.standard_normal((3, 8, 128)).astype(np.float32)
+    want, _ = cache.attend(q, 8, 0.09)
+    qd = torch.from_numpy(q).cuda()
+    size = P.attn_paged_workspace_bytes(cache.pages, 3, 8, cache.max_pages * 16)
+    streams = [torch.cuda.Stream().cuda_stream for _ in range(2)]
+    outs = [torch.zeros(3, 8, 128).cuda() for _ in range(8)]
+    spaces = [torch.empty(max(size, 16), dtype=torch.uint8).cuda() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        kw = {"workspace": spaces[i % 2], "workspace_bytes": size} if i < 4 else {}
+        P.attn_paged_dev(cache.pages, qd, out, cache.table, cache.lens_dev, 3, cache.max_pages, 8, 0.09, stream=streams[i % 2], **kw)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert np.array_equal(out.cpu().numpy().view(np.uint32), want.view(np.uint32))
+
+
+def test_long_sums_keep_f32_accuracy(P):
+    """A batch whose chunks are hundreds of units long, all keys of nearly equal weight: what the sums lose per unit must not
+    add up. Compared in 64 bits on the GPU, one head of each sequence."""
+    import torch
+
+    n, length, kv, d, page = 40, 16384, 2, 128, 64
+    gen = torch.Generator(device="cuda").manual_seed(27)
+    pages_per = length // page
+    k = torch.randn(n * pages_per, kv, page, d, generator=gen, device="cuda").half()
+    v = (torch.randn(n * pages_per, kv, page, d, generator=gen, device="cuda") + 0.25).half()
+    table = torch.arange(n * pages_per, dtype=torch.int32, device="cuda").reshape(n, pages_per).contiguous()
+    lens = torch.full((n,), length, dtype=torch.int32, device="cuda")
+    q = torch.randn(n, 8, d, generator=gen, device="cuda") * 0.3
+    out = torch.empty(n, 8, d, device="cuda")
+    pages = P.KvPages(P.KV_F16, k, v, None, None, n * pages_per, page, kv, d)
+    torch.cuda.synchronize()
+    P.attn_paged_dev(pages, q, out, table, lens, n, pages_per, 8, d ** -0.5)
+    P.synchronize()
+    err = ref = 0.0
+    for s in range(0, n, 7):
+        kk = k[table[s].long()].transpose(0, 1).reshape(kv, length, d).double()
+        vv = v[table[s].long()].transpose(0, 1).reshape(kv, length, d).double()
+        x = torch.einsum("gd,jd->gj", q[s, :4].double(), kk[0]) * d ** -0.5
+        want = torch.softmax(x, dim=1) @ vv[0]
+        err, ref = err + float((out[s, :4].double() - want).square().sum()), ref + float(want.square().sum())
+    assert (err / ref) ** 0.5 <= 48 * 2.0 ** -24
 
 
 def test_prompt_chunk_reads_its_cache_for_the_dense_attention(P):
