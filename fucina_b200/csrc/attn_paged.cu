@@ -13,12 +13,15 @@
 // shared-memory stages of one unit each, filled by cp.async and read by 1 to 4 warps, each with up to eight of the query
 // heads that share the kv head. A row that lies inside one chunk is finished there; pieces of rows that cross chunks go to
 // the workspace and a second kernel joins them in order. The chunks are fixed by the lengths, so a result does not depend on
-// which ring walked what. Small calls have one chunk per ring. Large ones give each ring one chunk of three quarters of its
-// fair share and hand out the rest in small ones as rings become free: SMs differ by a fifth in the rate at which memory
-// serves them (64 f16 sequences of up to 8000 tokens: equal shares took 137 to 195 us per SM). A first kernel then adds up
-// the lengths and clears the hand-out counter. When every row is short, each row has a team of rings, some of a CTA's, all of
-// them, or those of a cluster of CTAs, as the number of rows leaves room; their pieces are joined in (distributed) shared
-// memory, and that kernel is the only one. The lengths are read on the device: nothing on the host depends on them.
+// which ring walked what. Small calls have one chunk per ring. Large f16 ones, which memory bounds, give each ring one chunk
+// of three quarters of its fair share and hand out the rest in small ones as rings become free: SMs differ by a fifth in the
+// rate at which memory serves them (64 f16 sequences of up to 8000 tokens: with equal shares the first SM was done after 137
+// us, the last after 195; 193.6 us for the call against 198.1). A first kernel then adds up the lengths and clears the
+// hand-out counter. Q8_0 rings are bound by their own instructions and gain nothing (134 us with equal shares, 148 handed
+// out). When every row is short, each row has a team of rings, some of a CTA's, all of them, or those of a cluster of CTAs,
+// as the number of rows leaves room (one sequence of 517 tokens: 11.1 us by a CTA a row, 10.2 us by clusters of four); their
+// pieces are joined in (distributed) shared memory, and that kernel is the only one. The lengths are read on the device:
+// nothing on the host depends on them.
 //
 // Copies. The keys of a stage are refilled as soon as the scores are taken, the values after the second product: nearly
 // two units per ring are in flight at any time from two stages' room.
@@ -28,12 +31,17 @@
 // f32 value and the remainder (22 bits together), so query and weights are not rounded; the cache's f16 or int8 values are
 // exact in f16 (an int8 key, raised by 128, as a subnormal: its bits are the integer, and the sum begins with -128 times the
 // query's). Four heads fill the eight columns of an instruction (one tile of heads; a warp has one or two): with eight heads
-// as rows instead, groups of four heads, the usual ones, would leave half of every instruction and half of the softmax
-// empty. A lane holds one head of a tile throughout: its scores of keys g and g + 8, and its sums. Weights change from
+// as rows instead, groups of four heads, the usual ones, leave half of every instruction and half of the softmax empty (64
+// Q8_0 sequences of up to 8000 tokens: 152 us, 129 us with heads as columns). A lane holds one head of a tile throughout: its scores of keys g and g + 8, and its sums. Weights change from
 // sums to operands by movmatrix. Query rows are scaled by a power of two and weights by 2^15 (their maximum is 1) so that
 // remainders stay clear of f16's smallest steps. Q8_0: a key's scale multiplies the f32 sum of its 32-value block; a
 // value's scale s turns the two parts (a, b) of a weight into those of the product: a' = a s rounded, b' = b s + (a s - a'),
 // whose bracket is exact in f16.
+//
+// Measured (B200, 32 heads over 8 kv heads of 128): 64 sequences of 300 to 8000 tokens 198 us f16 = 5.50 TB/s, 84 % of a copy's
+// rate, and 124-131 us Q8_0 = 4.4-4.7 TB/s; one sequence of 131072 tokens, Q8_0, 67-70 us = 4.1-4.2 TB/s; of 8192 tokens, f16, 18.5 us; of
+// 517 tokens 9.8 us. The f16 form waits for memory; the Q8_0 form issues 960 warp instructions per unit, half an instruction
+// a cycle and scheduler, and waits for its own results; the small calls are launches and a chain of dependent loads.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -49,7 +57,7 @@ constexpr float kNegBig = -3.4e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSub = 16;       // keys that surely lie in one page
 constexpr int kTile = 4;       // query heads of a tile
-constexpr int kMaxRings = 16;  // 2 x kMaxRings pieces are joined by one lane each
+constexpr int kMaxRings = 16;
 constexpr int kSmemMost = 226 * 1024;
 constexpr size_t kMaxLen = (size_t)1 << 28;
 
@@ -140,7 +148,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 // The products of a unit join the running sums by f32 additions: the tensor instruction drops the bits of its sum that do not
 // fit, and over a chunk of some hundred instructions those losses, all towards zero, add up (64 f16 sequences of up to 8000
-// tokens: 1.7e-6 from the 64-bit result with the running sums inside the instruction, 0.7e-6 apart).
+// tokens: 1.7e-6 from the 64-bit result with the running sums inside the instruction, 0.5e-6 apart).
 __device__ __forceinline__ void add_to(float (&o)[4], const float (&c)[4]) {
     const float2 a = add2(make_float2(o[0], o[1]), make_float2(c[0], c[1])), b = add2(make_float2(o[2], o[3]), make_float2(c[2], c[3]));
     o[0] = a.x, o[1] = a.y, o[2] = b.x, o[3] = b.y;
@@ -620,26 +628,34 @@ __global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(c
                 }
             }
         } else {
-            float c[HT][UK / 16][4];
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                if (EXACT || kk < steps) {
+            for (int k0 = 0; k0 < KS; k0 += 4) {  // four instructions in a row, then an f32 addition (add_to)
+                if (EXACT || k0 < steps) {
+                    float c[HT][UK / 16][4];
 #pragma unroll
-                    for (int n = 0; n < UK / 16; ++n) {
-                        uint32_t r[4];
-                        ldsm_x4(ks + n * 16 * pitch + by_keys + kk * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
+                    for (int kk = k0; kk < k0 + 4; ++kk) {
+                        if (EXACT || kk < steps) {
 #pragma unroll
-                        for (int h = 0; h < HT; ++h) {
-                            if (kk == 0) mma16816_new(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
-                            else mma16816(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
+                            for (int n = 0; n < UK / 16; ++n) {
+                                uint32_t r[4];
+                                ldsm_x4(ks + n * 16 * pitch + by_keys + kk * 32, r);  // values 0-7 of the step: keys 0-7, 8-15; values 8-15: the same
+#pragma unroll
+                                for (int h = 0; h < HT; ++h) {
+                                    if (kk == k0) mma16816_new(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
+                                    else mma16816(c[h][n], r, qb[h][kk][0], qb[h][kk][1]);
+                                }
+                            }
                         }
                     }
+#pragma unroll
+                    for (int h = 0; h < HT; ++h)
+#pragma unroll
+                        for (int n = 0; n < UK / 16; ++n) {
+                            const float2 part_sum = make_float2(whole(c[h][n][0], c[h][n][1]), whole(c[h][n][2], c[h][n][3]));
+                            sc[h][n] = k0 == 0 ? part_sum : add2(sc[h][n], part_sum);
+                        }
                 }
             }
-#pragma unroll
-            for (int h = 0; h < HT; ++h)
-#pragma unroll
-                for (int n = 0; n < UK / 16; ++n) sc[h][n] = make_float2(whole(c[h][n][0], c[h][n][1]), whole(c[h][n][2], c[h][n][3]));
         }
         ring_sync();  // all the ring's warps are done with the keys
         if (left > 0) place(look);
@@ -1091,9 +1107,9 @@ struct Plan {
 constexpr int kMinUnits = 2, kMinUnitsDynamic = 3;
 
 // Teams walk rows of at most this many units per ring, longer ones are better spread over all rings: where the teams leave
-// SMs idle (one sequence of 4000 tokens, eight kv heads, f16: 19.5 us by teams of 24 rings, 5.3 units each, 15.5 us over all
-// rings; 8192 tokens 17.9 us over all rings, 22.1 us by teams of 48 rings in clusters of eight CTAs), and where they fill three
-// quarters of the GPU (16 sequences of 2000 tokens, Q8_0: 25.4 us by teams of 8 rings, 8 units each, 29.3 us over all rings).
+// SMs idle (one sequence of 4000 tokens, eight kv heads, f16: 18.5 us by teams of 24 rings, 5.3 units each, 15.0 us over all
+// rings), and where they fill three quarters of the GPU (16 sequences of 2000 tokens, Q8_0: 22.0 us by teams, 27.4 us over all
+// rings).
 constexpr int kTeamUnits = 4, kTeamUnitsFull = 8;
 
 int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max_len, int sm_count, Plan* out) {

@@ -16,6 +16,10 @@
 // neighbours lie further apart than twice the bound the 64-bit order is the same, and 64-bit arithmetic is needed for the
 // chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys. Rows whose
 // groups do not fall on whole lanes, or of more than 512 experts, are ranked on 64-bit keys in shared memory at once.
+//
+// Measured (B200): 4099 tokens over 256 experts, sigmoid, bias, four of eight groups: 37 us with 64-bit keys for every row, 15
+// us in this form, of which a row in doubt takes some 4 (the last of them ends the kernel); one token over 128 experts 5.2 us,
+// the launch.
 #include "internal.h"
 #include "runtime.h"
 
