@@ -17,7 +17,7 @@
 // of three quarters of its fair share and hand out the rest in small ones as rings become free: SMs differ by a fifth in the
 // rate at which memory serves them (64 f16 sequences of up to 8000 tokens: with equal shares the first SM was done after 137
 // us, the last after 195; 193.6 us for the call against 198.1). A first kernel then adds up the lengths and clears the
-// hand-out counter. Q8_0 rings are bound by their own instructions and gain nothing (134 us with equal shares, 148 handed
+// hand-out counter (the lengths alone where there are many sequences). Q8_0 rings are bound by their own instructions and gain nothing (134 us with equal shares, 148 handed
 // out). When every row is short, each row has a team of rings, some of a CTA's, all of them, or those of a cluster of CTAs,
 // as the number of rows leaves room (one sequence of 517 tokens: 11.1 us by a CTA a row, 10.2 us by clusters of four); their
 // pieces are joined in (distributed) shared memory, and that kernel is the only one. The lengths are read on the device:
@@ -84,7 +84,8 @@ struct PagedArgs {
     int stage_bytes;
     int row_mode;      // every row has a team of rings
     int team, cluster; // its rings in a CTA, and CTAs
-    int dynamic;       // the plan kernel has run: `sums` holds the units before each sequence, `next` counts handed-out chunks
+    int planned;       // the plan kernel has run: `sums` holds the units before each sequence
+    int dynamic;       // and `next` counts handed-out chunks
     int min_units;     // per chunk
     unsigned page_magic;                  // index of 16 keys / 16-key runs of a page = umulhi(index, page_magic); 0: one run a page
     unsigned page_chunks, scale_chunks;   // 16-byte chunks from page to page
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(c
     int count, chunk = blockIdx.x * A.rings + ring;
     auto units_total = [&]() {
         if (A.row_mode) return 1;
-        if (dynamic) return A.sums[A.n_seqs];
+        if (A.planned) return A.sums[A.n_seqs];
         int mine = 0;
         for (int s = lane; s < A.n_seqs; s += 32) {
             int first, end;
@@ -298,7 +299,7 @@ __global__ void __launch_bounds__(max_warps(DM, HT) * 32, 1) attn_paged_kernel(c
     const Cut split(A, units_total(), gridDim.x * A.rings);
     // unit `from` of all
     auto locate = [&](Cursor<UK>& c, int from) {
-        if (dynamic) {
+        if (A.planned) {
             // the last sequence with sums[s] <= from: 32 places at a time
             int lo = 0, hi = A.n_seqs;  // sums[lo] <= from < sums[hi]
             while (hi - lo > 1) {
@@ -1098,13 +1099,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const 
 // How a call is cut, from sizes the host knows.
 struct Plan {
     int dm, exact, tiles, passes, span, warps_per_ring, heads_per_warp, rings, stage_bytes;
-    int row_mode, team, cluster, dynamic, grid, chunks;
+    int row_mode, team, cluster, planned, dynamic, grid, chunks;
     size_t smem, sums_at, meta_at, parts_at, workspace;
 };
 
 // A chunk has at least two units (a ring's depth of copies; below that the joins cost more than the copies they spread),
 // three where chunks are handed out.
 constexpr int kMinUnits = 2, kMinUnitsDynamic = 3;
+
+// Up to this many sequences every ring adds up the lengths itself, 32 at a time, in less than the launch of a kernel that
+// does it for all; beyond, the plan kernel runs.
+constexpr size_t kPlanSeqs = 512;
+
 
 // Teams walk rows of at most this many units per ring, longer ones are better spread over all rings: where the teams leave
 // SMs idle (one sequence of 4000 tokens, eight kv heads, f16: 18.5 us by teams of 24 rings, 5.3 units each, 15.0 us over all
@@ -1132,7 +1138,7 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     if (p.rings * 2 * p.stage_bytes > kSmemMost) return fail(FQ_DECLINED_ARGS, "no shared-memory layout for d=%d and %d heads per kv head", d, group);
     p.smem = (size_t)p.rings * 2 * p.stage_bytes;
     const size_t rows = n_seqs * c.kv_heads * p.passes, units = max_len / keys + 2;
-    if (rows > (size_t)INT32_MAX / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
+    if (rows > ((size_t)INT32_MAX - 65536) / units) return fail(FQ_DECLINED_ARGS, "attention problem too large for one launch");
     // Teams: the most rings per row with which all rows run at once; whole CTAs where that leaves half the SMs idle, up to a
     // cluster of four (a team of 64 rings at most is joined by one warp).
     p.team = p.rings, p.cluster = 1;
@@ -1144,6 +1150,7 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     if (!p.row_mode) p.team = p.rings, p.cluster = 1;
     const size_t most = rows * units, rings_all = (size_t)sm_count * p.rings;
     p.dynamic = !p.row_mode && !q8 && most >= 48 * rings_all;
+    p.planned = !p.row_mode && (p.dynamic || n_seqs > kPlanSeqs);
     const size_t shares = (most + kMinUnits - 1) / kMinUnits, ctas = (shares + p.rings - 1) / p.rings;
     p.grid = p.row_mode ? (int)((rows + p.rings / p.team - 1) / (p.rings / p.team)) * p.cluster : (int)(ctas < (size_t)sm_count ? ctas : (size_t)sm_count);
     // one chunk per ring; handed out, the rest (a quarter of the fair shares) in chunks of an eighth of one or of three units:
@@ -1151,7 +1158,7 @@ int plan_paged(const KvView& c, bool q8, size_t n_seqs, size_t heads, size_t max
     p.chunks = p.grid * p.rings * (p.dynamic ? 6 : 1);
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.sums_at = 256;
-    p.meta_at = p.sums_at + (p.dynamic ? up((n_seqs + 1) * sizeof(int)) : 0);
+    p.meta_at = p.sums_at + (p.planned ? up((n_seqs + 1) * sizeof(int)) : 0);
     p.parts_at = p.meta_at + up(p.chunks * sizeof(int2));
     p.workspace = p.row_mode ? 0 : p.parts_at + (size_t)p.chunks * 2 * piece;
     *out = p;
@@ -1175,7 +1182,8 @@ cudaError_t launch_paged(const PagedArgs& a, const Plan& p, cudaStream_t st) {
     attr[0].val.clusterDim.x = (unsigned)p.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr, cfg.numAttrs = getenv("FUCINA_B200_NO_PDL") ? 1 : 2;
+    static const bool no_pdl = getenv("FUCINA_B200_NO_PDL") != nullptr;
+    cfg.attrs = attr, cfg.numAttrs = no_pdl ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, attn_paged_kernel<Q8, DM, EXACT, HT>, a);
 }
 template <bool Q8, int HT>
@@ -1255,14 +1263,14 @@ int fq_attn_paged_dev(const fq_kv_pages* pages, const float* q_dev, size_t q_str
     a.n_seqs = (int)n_seqs, a.max_pages = (int)max_pages, a.max_len = (int)max_len, a.heads = (int)heads, a.group = (int)heads / c.kv_heads;
     a.scale = scale, a.window = (int)window, a.out = out_dev, a.stats = stats_dev, a.status = ctx->status_dev;
     a.passes = p.passes, a.span = p.span, a.warps_per_ring = p.warps_per_ring, a.heads_per_warp = p.heads_per_warp, a.rows_per_warp = kTile * p.tiles;
-    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.team = p.team, a.cluster = p.cluster, a.dynamic = p.dynamic;
+    a.rings = p.rings, a.stage_bytes = p.stage_bytes, a.row_mode = p.row_mode, a.team = p.team, a.cluster = p.cluster, a.planned = p.planned, a.dynamic = p.dynamic;
     a.min_units = p.dynamic ? kMinUnitsDynamic : kMinUnits;
     const unsigned long long per_page = (unsigned long long)(c.page_tokens / kSub);
     a.page_magic = per_page == 1 ? 0 : (unsigned)(((1ull << 32) + per_page - 1) / per_page);  // exact below 2^32 / 256 runs of 16 keys
     a.page_chunks = (unsigned)(c.page_stride / (q8 ? 16 : 8)), a.scale_chunks = (unsigned)(c.scale_stride / 8);
     a.next = (int*)ws, a.sums = (int*)(ws + p.sums_at), a.meta = (int2*)(ws + p.meta_at), a.parts = (float*)(ws + p.parts_at);
     cudaError_t e = cudaSuccess;
-    if (p.dynamic) {
+    if (p.planned) {
         e = launch_pdl(unit_keys(p.dm) == 32 ? attn_paged_plan_kernel<32> : attn_paged_plan_kernel<16>, dim3(1), dim3(1024), 0, st, a);
         g_trace.launches++;
     }

@@ -204,7 +204,8 @@ FQ_API int fq_kv_read_dev(const fq_kv_pages* pages, void* k_out_dev, void* v_out
  * with lengths of their own): q_dev [n_seqs][heads][d] f32 with q_stride elements between sequences (0 = dense; a
  * multiple of 4), out_dev [n_seqs][heads][d] f32. Query head h reads kv head h / (heads / kv_heads). Sequence s sees
  * the keys [max(0, len - window), len) with len = kv_len_dev[s] (window 0: all; append the new token first, it counts).
- * out = softmax(scale * q.k) v, f32 accuracy throughout; a sequence of length 0 gets zeros. Optional stats_dev
+ * out = softmax(scale * q.k) v, f32 accuracy throughout; a sequence of length 0 gets zeros; out_dev overlaps no input.
+ * Optional stats_dev
  * [n_seqs][heads][2] = {row max, sum exp} (a length of 0: {-3.4e38, 0}).
  * max_len: the longest length that may occur (0 = max_pages * page_tokens); longer lengths count as max_len and leave
  * FQ_ERR_PAGE. It sizes the workspace and picks the split, so a replayed graph serves every length up to it.

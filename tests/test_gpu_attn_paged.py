@@ -412,3 +412,16 @@ def test_prompt_chunk_reads_its_cache_for_the_dense_attention(P):
         step, _ = cache.attend(q[n - 1:], heads, d ** -0.5)
         assert np.all(np.abs(step[0] - dense[n - 1]) <= np.maximum(2e-3 * np.abs(step[0]), 2e-3))
         check_attention(cache, [(k, v)], q[n - 1:], step, d ** -0.5)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8_0"])
+def test_thousands_of_sequences_of_every_length(P, kind):
+    """More sequences than a ring adds up by itself, a few long ones among them."""
+    rng = np.random.default_rng(28)
+    lens = [int(x) for x in rng.integers(0, 40, 1500)]
+    lens[7], lens[800], lens[1499] = 3000, 1700, 900
+    cache = Cache(P, kind, lens, 16, 1, 64, rng)
+    rows = cache.fill(rng)
+    q = rng.standard_normal((len(lens), 3, 64)).astype(np.float32)
+    got, stats = cache.attend(q, 3, 0.125, stats=True)
+    check_attention(cache, rows, q, got, 0.125, stats=stats)
