@@ -14,8 +14,8 @@
 // Bound: latency for a token, instruction issue for a batch (the logits are 4 bytes per 30 instructions). So a row is first
 // ranked on f32 keys whose error has a bound, in registers, a contiguous run of experts per lane; where the ranks'
 // neighbours lie further apart than twice the bound the 64-bit order is the same, and 64-bit arithmetic is needed for the
-// chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys. Rows whose
-// groups do not fall on whole lanes, or of more than 512 experts, are ranked on 64-bit keys in shared memory at once.
+// chosen scores alone. Otherwise (a few rows in a thousand, and ties) the row is ranked again on 64-bit keys. Rows of
+// more than 512 experts or 32 groups are ranked on 64-bit keys in shared memory at once.
 //
 // Measured (B200): 4099 tokens over 256 experts, sigmoid, bias, four of eight groups: 37 us with 64-bit keys for every row, 15
 // us in this form, of which a row in doubt takes some 4 (the last of them ends the kernel); one token over 128 experts 5.2 us,
@@ -35,6 +35,7 @@ struct RouterArgs {
     const float* logits;
     const float* bias;
     int rows, experts, k, sigmoid, groups, kept, top2, normalize;
+    int lanes;  // of a group, a power of two (see Place)
     float scale;
     int* selected;
     float* weights;
@@ -165,6 +166,20 @@ __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int la
     write_row(A, row, lane, sel_mine, w_mine);
 }
 
+// Which experts a lane holds: each group on `lanes` lanes of its own, NE consecutive experts a lane, in order. A group's last
+// lanes may be partly or wholly empty.
+template <int NE>
+struct Place {
+    int first, count;  // experts first .. first + count - 1
+    bool leader;       // the group's first lane
+    __device__ __forceinline__ Place(const RouterArgs& A, int lane) {
+        const int size = A.experts / A.groups, group = lane / A.lanes, at = (lane - group * A.lanes) * NE;
+        first = group * size + at;
+        count = group < A.groups ? max(0, min(NE, size - at)) : 0;
+        leader = group < A.groups && at == 0;
+    }
+};
+
 // The lane that holds the warp's largest value (0: none), the lowest of several: by the upper halves, then the lower ones.
 __device__ __forceinline__ int best_lane(unsigned long long mine) {
     const unsigned hi = (unsigned)(mine >> 32), top = __reduce_max_sync(0xffffffffu, hi);
@@ -176,15 +191,16 @@ __device__ __forceinline__ int best_lane(unsigned long long mine) {
     return __ffs(who) - 1;
 }
 
-// The same for NE consecutive experts per lane, in registers (experts v, groups of whole lanes).
+// A row ranked on 64-bit keys, NE experts per lane, in registers.
 template <int NE>
 __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int lane) {
     const float* x = A.logits + (size_t)row * A.experts;
     Scores sc{A.sigmoid != 0, -INFINITY, 1.0};
+    const Place<NE> mine(A, lane);
     float v[NE];
     double p[NE];
 #pragma unroll
-    for (int j = 0; j < NE; ++j) v[j] = lane * NE + j < A.experts ? x[lane * NE + j] : -INFINITY;
+    for (int j = 0; j < NE; ++j) v[j] = j < mine.count ? x[mine.first + j] : -INFINITY;
     if (!A.sigmoid) {
 #pragma unroll
         for (int j = 0; j < NE; ++j) sc.mx = fmaxf(sc.mx, v[j]);  // a NaN never wins
@@ -204,13 +220,12 @@ __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int la
     unsigned long long key[NE];
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
-        const int e = lane * NE + j;
         if (!A.sigmoid) p[j] /= sc.total;
         const bool closed = !(v[j] > -INFINITY);
-        key[j] = e >= A.experts ? kTaken : closed ? kClosed : ordered(p[j] + (A.bias ? (double)A.bias[e] : 0.0));
+        key[j] = j >= mine.count ? kTaken : closed ? kClosed : ordered(p[j] + (A.bias ? (double)A.bias[mine.first + j] : 0.0));
     }
     if (A.groups > 1) {
-        const int size = A.experts / A.groups, lanes = size / NE;
+        const int size = A.experts / A.groups, lanes = A.lanes;
         unsigned long long a = 0, b = 0;  // the two largest of the lane, then of the group's lanes
 #pragma unroll
         for (int j = 0; j < NE; ++j) {
@@ -222,8 +237,7 @@ __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int la
             const unsigned long long low = a < oa ? a : oa, second = b > ob ? b : ob;
             b = low > second ? low : second, a = a > oa ? a : oa;
         }
-        const bool leader = lane % lanes == 0 && lane * NE < A.experts;
-        unsigned long long rank = !leader ? kTaken : A.top2 && size > 1 ? ordered(key_of(a) + key_of(b)) : a;
+        unsigned long long rank = !mine.leader ? kTaken : A.top2 && size > 1 ? ordered(key_of(a) + key_of(b)) : a;
         unsigned open = 0;
         for (int r = 0; r < A.kept; ++r) {
             const int who = best_lane(rank);
@@ -246,7 +260,7 @@ __device__ __noinline__ void route_row_exact(const RouterArgs A, int row, int la
         for (int j = 1; j < NE; ++j)
             if (key[j] > top) top = key[j], at = j, pv = p[j];
         const int who = best_lane(top);
-        const int e = __shfl_sync(0xffffffffu, lane * NE + at, who);
+        const int e = __shfl_sync(0xffffffffu, mine.first + at, who);
         pv = __shfl_sync(0xffffffffu, pv, who);
         if (lane == s) sel_mine = e, w_mine = pv;
         if (lane == who) {
@@ -277,8 +291,7 @@ __device__ __forceinline__ int next_best(unsigned mine, float apart, float& prev
     return __ffs(who) - 1;
 }
 
-// NE consecutive experts per lane (NE = 0: every row on 64-bit keys); groups are whole lanes, 2^n of them, or absent.
-// A warp per row.
+// Up to NE experts per lane (NE = 0: every row on 64-bit keys in shared memory). A warp per row.
 template <int NE>
 __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constant__ RouterArgs A) {
     extern __shared__ unsigned long long router_smem[];
@@ -290,9 +303,10 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
         route_row_exact(A, row, lane, router_smem + (size_t)warp * A.experts);
     } else {
         const float* x = A.logits + (size_t)row * A.experts;
+        const Place<NE> mine(A, lane);
         float v[NE];
 #pragma unroll
-        for (int j = 0; j < NE; ++j) v[j] = lane * NE + j < A.experts ? x[lane * NE + j] : -INFINITY;
+        for (int j = 0; j < NE; ++j) v[j] = j < mine.count ? x[mine.first + j] : -INFINITY;
         unsigned key[NE];
         float apart, mx = 0.0f;
         bool sure = true;
@@ -306,10 +320,9 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
             float big = 0.0f;
 #pragma unroll
             for (int j = 0; j < NE; ++j) {
-                const int e = lane * NE + j;
                 const bool closed = !(v[j] > -INFINITY);  // NaN too
                 const float s = __fdividef(1.0f, 1.0f + __expf(-fmaxf(v[j], -80.0f)));
-                const float k = A.bias && e < A.experts ? s + A.bias[e] : s;
+                const float k = A.bias && j < mine.count ? s + A.bias[mine.first + j] : s;
                 key[j] = closed ? 0u : ordered32(k);
                 if (!closed) big = fmaxf(big, fabsf(k));
             }
@@ -330,8 +343,7 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
                 const float inv = 1.0f / sum;
 #pragma unroll
                 for (int j = 0; j < NE; ++j) {
-                    const int e = lane * NE + j;
-                    const float k = A.bias && e < A.experts ? p[j] * inv + A.bias[e] : p[j] * inv;
+                    const float k = A.bias && j < mine.count ? p[j] * inv + A.bias[mine.first + j] : p[j] * inv;
                     key[j] = v[j] > -INFINITY ? ordered32(k) : 0u;
                     if (v[j] > -INFINITY) big = fmaxf(big, fabsf(k));
                 }
@@ -344,8 +356,8 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
             }
         }
         if (A.groups > 1) {
-            // the two best of the lane, then of the group's lanes (a run of 2^n); ranks of closed groups stay in doubt
-            const int lanes = A.experts / A.groups / NE;
+            // the two best of the lane, then of the group's lanes; ranks of closed groups stay in doubt
+            const int lanes = A.lanes;
             float a = -INFINITY, b = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NE; ++j) {
@@ -357,22 +369,21 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
                 const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
                 b = fmaxf(fminf(a, oa), fmaxf(b, ob)), a = fmaxf(a, oa);
             }
-            const bool leader = lane % lanes == 0 && lane * NE < A.experts;
             const float rank = sums ? a + b : a;
-            unsigned mine = leader && rank > -INFINITY ? ordered32(rank) : 0u;
+            unsigned rank_mine = mine.leader && rank > -INFINITY ? ordered32(rank) : 0u;
             unsigned open = 0;  // lanes of open groups
-            const float far = mine && sums ? 2.0f * apart + 2.4e-7f * (fabsf(a) + fabsf(b)) : apart;
+            const float far = rank_mine && sums ? 2.0f * apart + 2.4e-7f * (fabsf(a) + fabsf(b)) : apart;
             const float apart_ranks = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(far)));
             float prev = INFINITY;
             for (int r = 0; r < A.kept + (A.kept < A.groups); ++r) {
-                const int who = next_best(mine, apart_ranks, prev);
+                const int who = next_best(rank_mine, apart_ranks, prev);
                 if (who < 0) {
                     sure = sure && who == -2 && r == A.kept;
                     break;
                 }
                 if (r < A.kept) {
                     open |= (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << who;
-                    if (lane == who) mine = 0u;
+                    if (lane == who) rank_mine = 0u;
                 }
             }
             if (!((open >> lane) & 1)) {
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(128) router_groups_kernel(const __grid_constan
                     sure = who == -2 && r == A.k;
                     break;
                 }
-                const int e = __shfl_sync(0xffffffffu, lane * NE + at, who);
+                const int e = __shfl_sync(0xffffffffu, mine.first + at, who);
                 xv = __shfl_sync(0xffffffffu, xv, who);
                 if (lane == r && r < A.k) sel_mine = e, v_mine = xv;
                 if (lane == who) {
@@ -439,15 +450,16 @@ extern "C" int fq_router_groups_dev(const float* logits_dev, size_t seq, size_t 
     std::lock_guard<std::recursive_mutex> g(g_dispatch_lock);
     g_trace.calls++;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    const RouterArgs a{logits_dev, bias_dev, (int)seq, (int)n_expert, (int)top_k, score == FQ_SCORE_SIGMOID, (int)n_group, (int)topk_group,
-                       group_score == FQ_GROUP_TOP2, normalize != 0, scale, selected_dev, weights_dev};
+    RouterArgs a{logits_dev, bias_dev, (int)seq, (int)n_expert, (int)top_k, score == FQ_SCORE_SIGMOID, (int)n_group, (int)topk_group,
+                       group_score == FQ_GROUP_TOP2, normalize != 0, 32, scale, selected_dev, weights_dev};
     const int warps = n_expert <= 1024 ? 4 : 1;  // eight bytes of shared memory per expert and warp, 32 KB at most
     const dim3 grid((unsigned)((seq + warps - 1) / warps)), block(warps * 32);
-    // experts per lane: the fewest that cover the row with every group on 2^n whole lanes
+    // experts per lane: the fewest with which every group has 2^n lanes of its own
     auto fits = [&](size_t ne) {
-        if (32 * ne < n_expert) return false;
-        const size_t size = n_expert / n_group, lanes = size / ne;
-        return n_group == 1 || (size % ne == 0 && (lanes & (lanes - 1)) == 0);
+        const size_t size = n_expert / n_group;
+        a.lanes = 1;
+        while (a.lanes * ne < size) a.lanes *= 2;
+        return a.lanes * n_group <= 32;
     };
     cudaError_t e;
     if (fits(2)) e = launch_pdl(router_groups_kernel<2>, grid, block, 0, st, a);
